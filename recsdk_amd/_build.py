@@ -18,7 +18,9 @@ LIB = os.path.join(HERE, "lib")
 OBJ = os.path.join(HERE, "lib", "obj")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
-HIP_SOURCES = ["hstu_abi.hip", "hstu_generic.hip", "hstu_mfma.hip", "hstu_mfma_fp8.hip", "hstu_backward.hip", "hstu_mfma_bwd.hip", "hstu_kvcache.hip", "hstu_kvcache_fp8.hip", "hstu_bias.hip", "hstu_layer.hip", "hstu_linear.hip", "hstu_linear_bwd.hip"]
+HIP_SOURCES = ["hstu_abi.hip", "hstu_generic.hip", "hstu_mfma.hip", "hstu_mfma_fp8.hip", "hstu_backward.hip", "hstu_mfma_bwd.hip", "hstu_kvcache.hip", "hstu_kvcache_fp8.hip", "hstu_bias.hip", "hstu_layer.hip", "hstu_linear.hip", "hstu_linear_bwd.hip",
+               "hstu_norm.hip", "hstu_pack8.hip", "hstu_gated.hip", "hstu_gemm_bf16.hip", "hstu_gemm_f16.hip", "hstu_gemm_f32.hip"]
+OPS_SOURCES = ["mxrec_hstu_ops.cpp", "mxrec_ffn_ops.cpp"]
 HIP_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fno-gpu-rdc",
              # packed fp32 VALU forms are kept out of every kernel in this library
              "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
@@ -85,7 +87,7 @@ def build_ops(verbose=False):
     tlib = os.path.join(os.path.dirname(torch.__file__), "lib")
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI),
            "-DUSE_ROCM", "-D__HIP_PLATFORM_AMD__", *inc, "-I", os.path.join(HERE, "..", "include"),
-           os.path.join(CSRC, "mxrec_hstu_ops.cpp"), "-o", ops_lib_path(),
+           *[os.path.join(CSRC, s) for s in OPS_SOURCES], "-o", ops_lib_path(),
            "-L", LIB, "-lhstu_hip", "-Wl,-rpath,$ORIGIN",
            "-L", tlib, "-ltorch", "-ltorch_cpu", "-lc10", "-ltorch_hip", "-lc10_hip", "-lamdhip64"]
     out = _run(cmd)

@@ -32,6 +32,10 @@ EXPORTS = [
     "hstu_hip_norm_multiply_dropout", "hstu_hip_norm_multiply_dropout_backward",
     "hstu_hip_norm_multiply_dropout_backward_get_workspace_size", "hstu_hip_in_linear_silu",
     "hstu_hip_in_linear_silu_backward", "hstu_hip_in_linear_silu_backward_get_workspace_size",
+    "hstu_hip_layer_norm", "hstu_hip_layer_norm_backward", "hstu_hip_layer_norm_backward_get_workspace_size",
+    "hstu_hip_activation_pack8", "hstu_hip_activation_unpack8",
+    "hstu_hip_gated_linear", "hstu_hip_gated_linear_get_workspace_size",
+    "hstu_hip_gated_linear_backward", "hstu_hip_gated_linear_backward_get_workspace_size",
 ]
 
 
@@ -142,6 +146,48 @@ class HstuInLinearSiluBwdParams(C.Structure):
     ]
 
 
+class HstuLayerNormParams(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("dtype", C.c_int32), ("param_dtype", C.c_int32), ("cols", C.c_int32), ("rows", C.c_int64),
+        ("x_stride", C.c_int64), ("eps", C.c_float), ("reserved", C.c_uint32), ("x", C.c_void_p), ("weight", C.c_void_p),
+        ("bias", C.c_void_p), ("y", C.c_void_p), ("mean", C.c_void_p), ("rstd", C.c_void_p),
+    ]
+
+
+class HstuLayerNormBwdParams(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("dtype", C.c_int32), ("param_dtype", C.c_int32), ("grad_dtype", C.c_int32),
+        ("rows", C.c_int64), ("cols", C.c_int32), ("reserved", C.c_uint32), ("x_stride", C.c_int64), ("dy_stride", C.c_int64),
+        ("d_y", C.c_void_p), ("x", C.c_void_p), ("weight", C.c_void_p), ("mean", C.c_void_p), ("rstd", C.c_void_p),
+        ("d_x", C.c_void_p), ("d_weight", C.c_void_p), ("d_bias", C.c_void_p),
+    ]
+
+
+class HstuPack8Params(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("dtype", C.c_int32), ("rows", C.c_int64), ("cols", C.c_int32), ("reserved", C.c_uint32),
+        ("x_stride", C.c_int64), ("x", C.c_void_p), ("codes", C.c_void_p), ("exponents", C.c_void_p),
+    ]
+
+
+class HstuGatedParams(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("dtype", C.c_int32), ("bias_dtype", C.c_int32), ("act", C.c_int32), ("keep", C.c_int32),
+        ("k", C.c_int32), ("f", C.c_int32), ("reserved", C.c_uint32), ("m", C.c_int64), ("x_stride", C.c_int64),
+        ("x", C.c_void_p), ("weight", C.c_void_p), ("bias", C.c_void_p), ("out", C.c_void_p), ("z", C.c_void_p),
+        ("z_exponents", C.c_void_p),
+    ]
+
+
+class HstuGatedBwdParams(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("dtype", C.c_int32), ("grad_bias_dtype", C.c_int32), ("act", C.c_int32), ("keep", C.c_int32),
+        ("k", C.c_int32), ("f", C.c_int32), ("reserved", C.c_uint32), ("m", C.c_int64), ("x_stride", C.c_int64),
+        ("dout_stride", C.c_int64), ("d_out", C.c_void_p), ("x", C.c_void_p), ("weight", C.c_void_p), ("z", C.c_void_p),
+        ("z_exponents", C.c_void_p), ("d_x", C.c_void_p), ("d_weight", C.c_void_p), ("d_bias", C.c_void_p),
+    ]
+
+
 _lib: Optional[C.CDLL] = None
 
 
@@ -179,6 +225,11 @@ def lib() -> C.CDLL:
         _lib.hstu_hip_norm_multiply_dropout_backward_get_workspace_size.argtypes = [C.POINTER(HstuNmdBwdParams), C.POINTER(C.c_uint64)]
         _lib.hstu_hip_rab_time_backward.argtypes = [C.POINTER(HstuRabTimeBwdParams), C.c_void_p]
         _lib.hstu_hip_rab_pos.argtypes = [C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.POINTER(C.c_int64), C.c_int32, C.c_void_p, C.c_void_p]
+        for n, t in (("layer_norm", HstuLayerNormParams), ("activation_pack8", HstuPack8Params), ("activation_unpack8", HstuPack8Params)):
+            getattr(_lib, f"hstu_hip_{n}").argtypes = [C.POINTER(t), C.c_void_p]
+        for n, t in (("layer_norm_backward", HstuLayerNormBwdParams), ("gated_linear", HstuGatedParams), ("gated_linear_backward", HstuGatedBwdParams)):
+            getattr(_lib, f"hstu_hip_{n}").argtypes = [C.POINTER(t), C.c_void_p, C.c_uint64, C.c_void_p]
+            getattr(_lib, f"hstu_hip_{n}_get_workspace_size").argtypes = [C.POINTER(t), C.POINTER(C.c_uint64)]
         _lib.hstu_hip_kv_token_positions.argtypes = [C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p]
     return _lib
 

@@ -1,0 +1,435 @@
+// The gated projection act(x Wg^T + bg) * (x Wu^T + bu) and its backward (mxrec::gated_linear): argument checks, the choice of
+// tiles, and the row work around the matrix products of hstu_gemm.h.
+//   forward   one product kernel whose waves hold a block of the gate and the matching block of the values, so that
+//             activation and product happen on the accumulators
+//   backward  dz from d_out and the kept z (one pass, also the column sums for d_bias), then d_x = dz W and d_weight = dz^T x,
+//             which read their operands as they lie in memory (transposing LDS reads; nothing is transposed in HBM)
+// dz is rounded to the I/O type between the two: the products run on the 16-bit matrix cores, and the rounding (2^-9 relative
+// per element, independent) averages out over sums of 2 f and of m terms.
+#include "hstu_ffn_common.h"
+#include "hstu_gemm.h"
+
+namespace hstu {
+
+// ---- rows to 16-byte boundaries ------------------------------------------------------------------------------------------
+// The product's copies move aligned 16-byte pieces.  An operand whose rows do not start on such boundaries, or end inside a
+// piece, is first copied to rows of `ld` elements, zeros behind each row.
+template <typename T>
+__global__ __launch_bounds__(256) void hstu_pad_rows_kernel(const T* src, int64_t stride, int64_t rows, int cols, T* dst, int64_t ld) {
+    const int per_row = (int)(ld / 8 + (ld % 8 ? 1 : 0));   // pieces of 8 elements
+    const int64_t n = rows * per_row;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / per_row;
+        const int c = (int)(i - r * per_row) * 8;
+        float v[8];
+        load8_any(src + r * stride + (cols - c > 0 ? c : 0), cols - c, v);
+        store8_any(dst + r * ld + c, (int)(ld - c), v);
+    }
+}
+
+// ---- dz ------------------------------------------------------------------------------------------------------------------
+// A lane works on 8 consecutive columns of both halves and walks down its rows; `lanes` lanes side by side, 256 / lanes rows
+// at a time.  HBM-bound: reads d_out and z, writes dz.  Columns [2 f, ld) of dz are set to zero (the product reads them).
+struct DzArgs {
+    const void* d_out;
+    const void* z;
+    const uint8_t* z_exp;
+    void* dz;              // [m, ld], or NULL
+    float* partial;        // [row blocks, 2 f] column sums, or NULL
+    int64_t m, dout_stride, ld;
+    int64_t rows_wg;       // rows of a workgroup
+    int32_t f, act, keep, lanes, col_blocks;
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void hstu_gated_dz_kernel(const DzArgs a) {
+    __shared__ float red[16][256 + 4];   // 16 columns of each of the 256 lanes
+    const int lanes = a.lanes, tx = threadIdx.x & (lanes - 1), ty = threadIdx.x / lanes, step = 256 / lanes;
+    const int cb = blockIdx.x % a.col_blocks;
+    const int64_t rb = blockIdx.x / a.col_blocks;
+    const int c = (cb * lanes + tx) * 8, n = a.f - c;
+    const int64_t r0 = rb * a.rows_wg, r1 = min(r0 + a.rows_wg, a.m);
+    const int groups = (a.f + HSTU_PACK8_GROUP - 1) / HSTU_PACK8_GROUP;
+    float sg[8], su[8];
+#pragma unroll
+    for (int k = 0; k < 8; k++) sg[k] = su[k] = 0.f;
+    if (n > 0) {
+        for (int64_t r = r0 + ty; r < r1; r += step) {
+            float d[8], zg[8], zu[8];
+            load8_any(reinterpret_cast<const T*>(a.d_out) + r * a.dout_stride + c, n, d);
+            if (a.keep == HSTU_KEEP_8BIT) {
+                const uint8_t* z = reinterpret_cast<const uint8_t*>(a.z) + r * 2 * a.f + c;
+                const uint8_t* e = a.z_exp + r * 2 * groups + c / HSTU_PACK8_GROUP;
+                unpack8_any(z, n, e[0], largest_finite<float>(), zg);
+                unpack8_any(z + a.f, n, e[groups], largest_finite<float>(), zu);
+            } else {
+                const T* z = reinterpret_cast<const T*>(a.z) + r * 2 * a.f + c;
+                load8_any(z, n, zg);
+                load8_any(z + a.f, n, zu);
+            }
+            float dg[8], du[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                float act, grad;
+                act_and_grad(zg[k], a.act, act, grad);
+                dg[k] = d[k] * zu[k] * grad;
+                du[k] = d[k] * act;
+                sg[k] += dg[k];
+                su[k] += du[k];
+            }
+            if (a.dz) {
+                T* dz = reinterpret_cast<T*>(a.dz) + r * a.ld + c;
+                store8_any(dz, n, dg);
+                store8_any(dz + a.f, n, du);
+                if (n <= 8)
+                    for (int64_t k = 2 * (int64_t)a.f; k < a.ld; k++) reinterpret_cast<T*>(a.dz)[r * a.ld + k] = from_float<T>(0.f);
+            }
+        }
+    }
+    if (!a.partial) return;
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+        red[k][threadIdx.x] = sg[k];
+        red[8 + k][threadIdx.x] = su[k];
+    }
+    __syncthreads();
+    // column j of lane t: rows of the workgroup in order
+    for (int i = threadIdx.x; i < lanes * 16; i += 256) {
+        const int t = i >> 4, j = i & 15, col = (cb * lanes + t) * 8 + (j & 7);
+        if (col >= a.f) continue;
+        float s = 0.f;
+        for (int y = 0; y < step; y++) s += red[j][y * lanes + t];
+        a.partial[rb * 2 * a.f + (j >= 8 ? a.f : 0) + col] = s;
+    }
+}
+
+// ---- sums over the shares of a contraction -------------------------------------------------------------------------------
+template <typename T>
+__global__ __launch_bounds__(256) void hstu_sum_splits_kernel(const float* partial, int splits, int64_t n, T* out) {
+    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (int64_t)gridDim.x * 1024) {
+        if (i + 4 <= n) {
+            typedef gm_f32x4 __attribute__((aligned(4))) f4;
+            gm_f32x4 s = *reinterpret_cast<const f4*>(partial + i);
+            for (int k = 1; k < splits; k++) s += *reinterpret_cast<const f4*>(partial + k * n + i);
+#pragma unroll
+            for (int k = 0; k < 4; k++) out[i + k] = from_float<T>(s[k]);
+        } else {
+            for (int64_t j = i; j < n; j++) {
+                float s = partial[j];
+                for (int k = 1; k < splits; k++) s += partial[k * n + j];
+                out[j] = from_float<T>(s);
+            }
+        }
+    }
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------------
+static int elem_bytes(int32_t dtype) { return dtype == HSTU_F32 ? 4 : 2; }
+static uint64_t up256(uint64_t v) { return (v + 255) / 256 * 256; }
+static int64_t padded(int64_t cols, int32_t dtype) {
+    const int e = 16 / elem_bytes(dtype);
+    return (cols + e - 1) / e * e;
+}
+static bool needs_pad(const void* p, int64_t stride, int64_t cols, int32_t dtype) {
+    const int e = 16 / elem_bytes(dtype);
+    // (a tile's copies address up to 256 rows with 31 bits: rows further apart than 2^20 elements are brought together too)
+    return (reinterpret_cast<uintptr_t>(p) & 15) || stride % e || cols % e || stride > (1 << 20);
+}
+static bool bad_align(const void* p, int32_t dtype) { return (reinterpret_cast<uintptr_t>(p) & (dtype == HSTU_F32 ? 3 : 1)) != 0; }
+
+static hipError_t launch_gemm(int32_t dtype, const GemmArgs& a, int kind, int tile, hipStream_t st) {
+    if (dtype == HSTU_F32) return launch_gemm_f32(a, kind, tile, st);
+    if (dtype == HSTU_F16) return launch_gemm_f16(a, kind, tile, st);
+    return launch_gemm_bf16(a, kind, tile, st);
+}
+
+struct Plan { int tile, splits, tiles_n, tiles_m; int64_t c_split; };
+
+// Tiles and shares of the contraction.  256 x 256 tiles where they fill the chip, 128 x 128 ones otherwise, and a plain
+// product's contraction is cut (in shares of at least 512) while there are fewer workgroups than CUs.
+static Plan gemm_plan(int kind, int32_t dtype, int64_t M, int64_t N, int64_t C) {
+    Plan p;
+    auto tiles = [&](int t, int64_t& tm, int64_t& tn) {
+        tm = (M + gemm_tile_m(t) - 1) / gemm_tile_m(t);
+        tn = (N + gemm_tile_n(t, kind) - 1) / gemm_tile_n(t, kind);
+    };
+    int64_t tm, tn;
+    tiles(TILE_256, tm, tn);
+    p.tile = TILE_256;
+    if (tm * tn < 192) {
+        p.tile = TILE_128;
+        tiles(TILE_128, tm, tn);
+    }
+    p.tiles_m = (int)tm;
+    p.tiles_n = (int)tn;
+    p.splits = 1;
+    const int64_t bk = 128 / elem_bytes(dtype);
+    if (kind != GEMM_GATED) {
+        while (p.splits < 64 && tm * tn * p.splits * 2 <= 512 && C / (p.splits * 2) >= 512) p.splits *= 2;
+    }
+    const int64_t pieces = (C + bk - 1) / bk;
+    p.c_split = (pieces + p.splits - 1) / p.splits * bk;
+    p.splits = C > 0 ? (int)((C + p.c_split - 1) / p.c_split) : 1;
+    if (p.c_split == 0) p.c_split = bk;
+    return p;
+}
+
+static int gemm_too_large(const Plan& p) {
+    if ((int64_t)p.tiles_m * p.tiles_n * p.splits > 0x7fffffffLL) return fail(HSTU_ERR_UNSUPPORTED, "m * f too large for one launch");
+    return HSTU_OK;
+}
+
+static void fill(GemmArgs& a, const Plan& pl, int64_t M, int64_t N, int64_t C) {
+    a.M = M; a.N = (int32_t)N; a.C = C;
+    a.c_split = pl.c_split; a.splits = pl.splits; a.tiles_m = pl.tiles_m; a.tiles_n = pl.tiles_n;
+}
+
+static hipError_t launch_pad(int32_t dtype, const void* src, int64_t stride, int64_t rows, int cols, void* dst, int64_t ld, hipStream_t st) {
+    if (rows == 0) return hipSuccess;
+    const int64_t want = (rows * ((ld + 7) / 8) + 255) / 256;
+    const dim3 grid((unsigned)(want > 4096 ? 4096 : want));
+    if (dtype == HSTU_F32) hipLaunchKernelGGL(hstu_pad_rows_kernel<float>, grid, dim3(256), 0, st, (const float*)src, stride, rows, cols, (float*)dst, ld);
+    else if (dtype == HSTU_F16) hipLaunchKernelGGL(hstu_pad_rows_kernel<_Float16>, grid, dim3(256), 0, st, (const _Float16*)src, stride, rows, cols, (_Float16*)dst, ld);
+    else hipLaunchKernelGGL(hstu_pad_rows_kernel<__bf16>, grid, dim3(256), 0, st, (const __bf16*)src, stride, rows, cols, (__bf16*)dst, ld);
+    return hipGetLastError();
+}
+
+static int gated_check_sizes(int32_t dtype, int32_t act, int32_t keep, int64_t m, int32_t k, int32_t f) {
+    if (dtype != HSTU_F32 && dtype != HSTU_F16 && dtype != HSTU_BF16)
+        return fail(HSTU_ERR_INVALID_ARGUMENT, "dtype expect float32, float16 or bfloat16, but value is %d", dtype);
+    if (act != HSTU_ACT_SILU && act != HSTU_ACT_GELU) return fail(HSTU_ERR_INVALID_ARGUMENT, "act expect 0 (silu) or 1 (gelu), but value is %d", act);
+    if (keep != HSTU_KEEP_NONE && keep != HSTU_KEEP_FULL && keep != HSTU_KEEP_8BIT) return fail(HSTU_ERR_INVALID_ARGUMENT, "keep expect 0, 1 or 2, but value is %d", keep);
+    if (keep == HSTU_KEEP_8BIT && dtype == HSTU_F32) return fail(HSTU_ERR_INVALID_ARGUMENT, "8-bit checkpoints need float16 or bfloat16");
+    if (m < 0 || m > HSTU_FFN_MAX_ROWS) return fail(HSTU_ERR_INVALID_ARGUMENT, "x dim0 must in range:[0,%lld].", HSTU_FFN_MAX_ROWS);
+    if (k < 1 || k > HSTU_GATED_MAX_K) return fail(HSTU_ERR_INVALID_ARGUMENT, "x dim1 must in range:[1,%d].", HSTU_GATED_MAX_K);
+    if (f < 1 || f > HSTU_GATED_MAX_F) return fail(HSTU_ERR_INVALID_ARGUMENT, "weight dim0 must be twice a number in range:[1,%d].", HSTU_GATED_MAX_F);
+    return HSTU_OK;
+}
+
+struct GatedLayout { uint64_t x, w, bytes; bool pad_x, pad_w; };
+static GatedLayout gated_layout(const hstu_gated_params* p) {
+    GatedLayout l;
+    const uint64_t e = elem_bytes(p->dtype), ld = padded(p->k, p->dtype);
+    l.pad_x = p->m > 0 && needs_pad(p->x, p->m > 1 ? p->x_stride : ld, p->k, p->dtype);
+    l.pad_w = p->m > 0 && needs_pad(p->weight, p->k, p->k, p->dtype);
+    l.x = 0;
+    l.w = l.pad_x ? up256(p->m * ld * e) : 0;
+    l.bytes = l.w + (l.pad_w ? up256(2 * (uint64_t)p->f * ld * e) : 0);
+    return l;
+}
+
+static int gated_validate(const hstu_gated_params* p) {
+    if (!p) return fail(HSTU_ERR_INVALID_ARGUMENT, "params is NULL");
+    if (p->struct_size != sizeof(hstu_gated_params))
+        return fail(HSTU_ERR_INVALID_ARGUMENT, "hstu_gated_params size mismatch: caller %u, library %zu", p->struct_size, sizeof(hstu_gated_params));
+    const int rc = gated_check_sizes(p->dtype, p->act, p->keep, p->m, p->k, p->f);
+    if (rc != HSTU_OK) return rc;
+    if (p->bias_dtype != p->dtype && p->bias_dtype != HSTU_F32) return fail(HSTU_ERR_INVALID_ARGUMENT, "bias_dtype expect float32 or the dtype of x, but value is %d", p->bias_dtype);
+    if (p->x_stride < 0) return fail(HSTU_ERR_INVALID_ARGUMENT, "x_stride must not be negative");
+    if (p->m == 0) return HSTU_OK;
+    if (!p->x || !p->weight || !p->out) return fail(HSTU_ERR_INVALID_ARGUMENT, "x, weight and out must not be NULL");
+    if ((p->keep != HSTU_KEEP_NONE && !p->z) || (p->keep == HSTU_KEEP_8BIT && !p->z_exponents))
+        return fail(HSTU_ERR_INVALID_ARGUMENT, "z (and z_exponents for 8 bits) must not be NULL when they are kept");
+    if (bad_align(p->x, p->dtype) || bad_align(p->weight, p->dtype) || bad_align(p->out, p->dtype) || bad_align(p->bias, p->bias_dtype) ||
+        (p->keep == HSTU_KEEP_FULL && bad_align(p->z, p->dtype)))
+        return fail(HSTU_ERR_UNSUPPORTED, "x, weight, bias, out and z must be aligned to their element types");
+    return HSTU_OK;
+}
+
+struct GatedBwdLayout {
+    Plan dx, dw;
+    int64_t ld, kld;                 // rows of dz, padded rows of x / weight
+    bool need_dz, pad_x, pad_w;
+    uint64_t dz, x, w, parts, sums, bytes;
+    int lanes, col_blocks;
+    int64_t rows_wg, row_blocks;
+};
+
+static GatedBwdLayout gated_bwd_layout(const hstu_gated_bwd_params* p) {
+    GatedBwdLayout l;
+    const uint64_t e = elem_bytes(p->dtype);
+    l.ld = padded(2 * (int64_t)p->f, p->dtype);
+    l.kld = padded(p->k, p->dtype);
+    l.need_dz = p->d_x || p->d_weight;
+    l.pad_x = p->d_weight && p->m > 0 && needs_pad(p->x, p->m > 1 ? p->x_stride : l.kld, p->k, p->dtype);
+    l.pad_w = p->d_x && p->m > 0 && needs_pad(p->weight, p->k, p->k, p->dtype);
+    l.dx = gemm_plan(GEMM_DX, p->dtype, p->m, p->k, 2 * (int64_t)p->f);
+    l.dw = gemm_plan(GEMM_DW, p->dtype, 2 * (int64_t)p->f, p->k, p->m);
+    // about 2048 workgroups, but at least four rows a lane where there are as many
+    l.lanes = 8;
+    while (l.lanes < 64 && l.lanes * 8 < p->f) l.lanes *= 2;
+    l.col_blocks = (p->f + l.lanes * 8 - 1) / (l.lanes * 8);
+    const int64_t step = 256 / l.lanes;
+    int64_t rows = (p->m * l.col_blocks + 2047) / 2048;
+    rows = (rows + step - 1) / step * step;
+    l.rows_wg = rows < 4 * step ? 4 * step : rows;
+    l.row_blocks = (p->m + l.rows_wg - 1) / l.rows_wg;
+    if (l.row_blocks < 1) l.row_blocks = 1;
+    uint64_t at = 0;
+    l.dz = at;
+    if (l.need_dz) at += up256((uint64_t)p->m * l.ld * e);
+    l.x = at;
+    if (l.pad_x) at += up256((uint64_t)p->m * l.kld * e);
+    l.w = at;
+    if (l.pad_w) at += up256(2 * (uint64_t)p->f * l.kld * e);
+    l.parts = at;
+    uint64_t parts = 0;
+    if (p->d_x && l.dx.splits > 1) parts = (uint64_t)l.dx.splits * p->m * p->k * 4;
+    if (p->d_weight && l.dw.splits > 1) { const uint64_t q = (uint64_t)l.dw.splits * 2 * p->f * p->k * 4; parts = q > parts ? q : parts; }
+    at += up256(parts);
+    l.sums = at;
+    if (p->d_bias) at += up256((uint64_t)l.row_blocks * 2 * p->f * 4);
+    l.bytes = at;
+    return l;
+}
+
+static int gated_bwd_validate(const hstu_gated_bwd_params* p) {
+    if (!p) return fail(HSTU_ERR_INVALID_ARGUMENT, "params is NULL");
+    if (p->struct_size != sizeof(hstu_gated_bwd_params))
+        return fail(HSTU_ERR_INVALID_ARGUMENT, "hstu_gated_bwd_params size mismatch: caller %u, library %zu", p->struct_size, sizeof(hstu_gated_bwd_params));
+    const int rc = gated_check_sizes(p->dtype, p->act, p->keep, p->m, p->k, p->f);
+    if (rc != HSTU_OK) return rc;
+    if (p->keep == HSTU_KEEP_NONE) return fail(HSTU_ERR_INVALID_ARGUMENT, "keep expect 1 or 2, but value is 0");
+    if (p->grad_bias_dtype != p->dtype && p->grad_bias_dtype != HSTU_F32)
+        return fail(HSTU_ERR_INVALID_ARGUMENT, "grad_bias_dtype expect float32 or the dtype of x, but value is %d", p->grad_bias_dtype);
+    if (p->x_stride < 0 || p->dout_stride < 0) return fail(HSTU_ERR_INVALID_ARGUMENT, "x_stride and dout_stride must not be negative");
+    if (p->m > 0) {
+        if (!p->d_out || !p->z || (p->keep == HSTU_KEEP_8BIT && !p->z_exponents))
+            return fail(HSTU_ERR_INVALID_ARGUMENT, "d_out and z (and z_exponents for 8 bits) must not be NULL");
+        if ((p->d_weight && !p->x) || (p->d_x && !p->weight)) return fail(HSTU_ERR_INVALID_ARGUMENT, "x (for d_weight) and weight (for d_x) must not be NULL");
+    }
+    if (bad_align(p->d_out, p->dtype) || bad_align(p->x, p->dtype) || bad_align(p->weight, p->dtype) || bad_align(p->d_x, p->dtype) ||
+        bad_align(p->d_weight, p->dtype) || bad_align(p->d_bias, p->grad_bias_dtype) || (p->keep == HSTU_KEEP_FULL && bad_align(p->z, p->dtype)))
+        return fail(HSTU_ERR_UNSUPPORTED, "d_out, x, weight, z and the gradients must be aligned to their element types");
+    return HSTU_OK;
+}
+
+static int check_workspace(void* ws, uint64_t have, uint64_t need) {
+    if (need && (!ws || have < need || (reinterpret_cast<uintptr_t>(ws) & 15)))
+        return fail(HSTU_ERR_WORKSPACE, "workspace of %llu bytes (16-byte aligned) needed, got %llu at %p", (unsigned long long)need, (unsigned long long)have, ws);
+    return HSTU_OK;
+}
+
+static hipError_t sum_splits(int32_t dtype, const float* partial, int splits, int64_t n, void* out, hipStream_t st) {
+    const int64_t want = (n + 1023) / 1024;
+    const dim3 grid((unsigned)(want > 4096 ? 4096 : want));
+    if (dtype == HSTU_F32) hipLaunchKernelGGL(hstu_sum_splits_kernel<float>, grid, dim3(256), 0, st, partial, splits, n, (float*)out);
+    else if (dtype == HSTU_F16) hipLaunchKernelGGL(hstu_sum_splits_kernel<_Float16>, grid, dim3(256), 0, st, partial, splits, n, (_Float16*)out);
+    else hipLaunchKernelGGL(hstu_sum_splits_kernel<__bf16>, grid, dim3(256), 0, st, partial, splits, n, (__bf16*)out);
+    return hipGetLastError();
+}
+
+}  // namespace hstu
+
+using namespace hstu;
+
+extern "C" int hstu_hip_gated_linear_get_workspace_size(const hstu_gated_params* p, uint64_t* bytes) {
+    if (!bytes) return fail(HSTU_ERR_INVALID_ARGUMENT, "workspace_bytes is NULL");
+    const int rc = gated_validate(p);
+    if (rc != HSTU_OK) return rc;
+    *bytes = gated_layout(p).bytes;
+    return HSTU_OK;
+}
+
+extern "C" int hstu_hip_gated_linear(const hstu_gated_params* p, void* workspace, uint64_t workspace_bytes, void* stream) {
+    int rc = gated_validate(p);
+    if (rc != HSTU_OK || p->m == 0) return rc;
+    const GatedLayout l = gated_layout(p);
+    rc = check_workspace(workspace, workspace_bytes, l.bytes);
+    if (rc != HSTU_OK) return rc;
+    const Plan pl = gemm_plan(GEMM_GATED, p->dtype, p->m, p->f, p->k);
+    rc = gemm_too_large(pl);
+    if (rc != HSTU_OK) return rc;
+    hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    char* ws = reinterpret_cast<char*>(workspace);
+    const int64_t ld = padded(p->k, p->dtype);
+    hipError_t e = hipSuccess;
+    if (l.pad_x) e = launch_pad(p->dtype, p->x, p->x_stride, p->m, p->k, ws + l.x, ld, st);
+    if (e == hipSuccess && l.pad_w) e = launch_pad(p->dtype, p->weight, p->k, 2 * (int64_t)p->f, p->k, ws + l.w, ld, st);
+    if (e == hipSuccess) {
+        GemmArgs a = {};
+        fill(a, pl, p->m, p->f, p->k);
+        a.n_op = l.pad_w ? ws + l.w : p->weight;
+        a.n_ld = l.pad_w ? ld : p->k;
+        a.m_op = l.pad_x ? ws + l.x : p->x;
+        a.m_ld = l.pad_x ? ld : p->m > 1 ? p->x_stride : ld;
+        a.out = p->out;
+        a.bias = p->bias;
+        a.bias_f32 = p->bias_dtype == HSTU_F32;
+        a.act = p->act;
+        a.keep = p->keep;
+        a.z = p->z;
+        a.z_exp = p->z_exponents;
+        e = launch_gemm(p->dtype, a, GEMM_GATED, pl.tile, st);
+    }
+    if (e != hipSuccess) return fail(HSTU_ERR_LAUNCH, "kernel launch failed: %s", hipGetErrorString(e));
+    return HSTU_OK;
+}
+
+extern "C" int hstu_hip_gated_linear_backward_get_workspace_size(const hstu_gated_bwd_params* p, uint64_t* bytes) {
+    if (!bytes) return fail(HSTU_ERR_INVALID_ARGUMENT, "workspace_bytes is NULL");
+    const int rc = gated_bwd_validate(p);
+    if (rc != HSTU_OK) return rc;
+    *bytes = gated_bwd_layout(p).bytes;
+    return HSTU_OK;
+}
+
+extern "C" int hstu_hip_gated_linear_backward(const hstu_gated_bwd_params* p, void* workspace, uint64_t workspace_bytes, void* stream) {
+    int rc = gated_bwd_validate(p);
+    if (rc != HSTU_OK) return rc;
+    const GatedBwdLayout l = gated_bwd_layout(p);
+    rc = check_workspace(workspace, workspace_bytes, l.bytes);
+    if (rc != HSTU_OK) return rc;
+    if (p->d_x && (rc = gemm_too_large(l.dx)) != HSTU_OK) return rc;
+    if (p->d_weight && (rc = gemm_too_large(l.dw)) != HSTU_OK) return rc;
+    hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    char* ws = reinterpret_cast<char*>(workspace);
+    hipError_t e = hipSuccess;
+    if (l.need_dz || p->d_bias) {
+        DzArgs d = {};
+        d.d_out = p->d_out; d.z = p->z; d.z_exp = p->z_exponents;
+        d.dz = l.need_dz ? ws + l.dz : nullptr;
+        d.partial = p->d_bias ? reinterpret_cast<float*>(ws + l.sums) : nullptr;
+        d.m = p->m; d.dout_stride = p->dout_stride; d.ld = l.ld; d.rows_wg = l.rows_wg;
+        d.f = p->f; d.act = p->act; d.keep = p->keep; d.lanes = l.lanes; d.col_blocks = l.col_blocks;
+        const int64_t blocks = l.row_blocks * l.col_blocks;
+        if (blocks > 0x7fffffffLL) return fail(HSTU_ERR_UNSUPPORTED, "m * f too large for one launch");
+        // without rows the workgroups write zero sums
+        const dim3 grid((unsigned)blocks);
+        if (p->dtype == HSTU_F32) hipLaunchKernelGGL(hstu_gated_dz_kernel<float>, grid, dim3(256), 0, st, d);
+        else if (p->dtype == HSTU_F16) hipLaunchKernelGGL(hstu_gated_dz_kernel<_Float16>, grid, dim3(256), 0, st, d);
+        else hipLaunchKernelGGL(hstu_gated_dz_kernel<__bf16>, grid, dim3(256), 0, st, d);
+        e = hipGetLastError();
+        if (e == hipSuccess && p->d_bias) {
+            char* db = reinterpret_cast<char*>(p->d_bias);
+            e = launch_colsum(d.partial, (int)l.row_blocks, p->f, db, db + (int64_t)p->f * elem_bytes(p->grad_bias_dtype), p->grad_bias_dtype, st);
+        }
+    }
+    if (e == hipSuccess && l.pad_w) e = launch_pad(p->dtype, p->weight, p->k, 2 * (int64_t)p->f, p->k, ws + l.w, l.kld, st);
+    if (e == hipSuccess && l.pad_x) e = launch_pad(p->dtype, p->x, p->x_stride, p->m, p->k, ws + l.x, l.kld, st);
+    if (e == hipSuccess && p->d_x && p->m > 0) {
+        GemmArgs a = {};
+        fill(a, l.dx, p->m, p->k, 2 * (int64_t)p->f);
+        a.n_op = l.pad_w ? ws + l.w : p->weight;
+        a.n_ld = l.pad_w ? l.kld : p->k;
+        a.m_op = ws + l.dz;
+        a.m_ld = l.ld;
+        a.out = l.dx.splits > 1 ? ws + l.parts : p->d_x;
+        e = launch_gemm(p->dtype, a, GEMM_DX, l.dx.tile, st);
+        if (e == hipSuccess && l.dx.splits > 1) e = sum_splits(p->dtype, reinterpret_cast<float*>(ws + l.parts), l.dx.splits, p->m * p->k, p->d_x, st);
+    }
+    if (e == hipSuccess && p->d_weight) {
+        // without rows the product of empty sums writes zeros
+        GemmArgs a = {};
+        fill(a, l.dw, 2 * (int64_t)p->f, p->k, p->m);
+        a.n_op = l.pad_x ? ws + l.x : p->x;
+        a.n_ld = l.pad_x ? l.kld : p->m > 1 ? p->x_stride : l.kld;
+        a.m_op = ws + l.dz;
+        a.m_ld = l.ld;
+        a.out = l.dw.splits > 1 ? ws + l.parts : p->d_weight;
+        e = launch_gemm(p->dtype, a, GEMM_DW, l.dw.tile, st);
+        if (e == hipSuccess && l.dw.splits > 1) e = sum_splits(p->dtype, reinterpret_cast<float*>(ws + l.parts), l.dw.splits, 2 * (int64_t)p->f * p->k, p->d_weight, st);
+    }
+    if (e != hipSuccess) return fail(HSTU_ERR_LAUNCH, "kernel launch failed: %s", hipGetErrorString(e));
+    return HSTU_OK;
+}
