@@ -145,33 +145,40 @@ static hipError_t launch_gemm(int32_t dtype, const GemmArgs& a, int kind, int ti
 
 struct Plan { int tile, splits, tiles_n, tiles_m; int64_t c_split; };
 
-// Tiles and shares of the contraction.  256 x 256 tiles where they fill the chip, 128 x 128 ones otherwise, and a plain
-// product's contraction is cut (in shares of at least 512) while there are fewer workgroups than CUs.
+// Tiles and shares of the contraction: the cheapest by a model of the launch, in microseconds.  A workgroup takes a start and an
+// end (`fixed`) and `piece` for each piece of its share; workgroups come in rounds of what the chip holds at a time; shares
+// beyond one cost a second kernel that adds their fp32 sums.
+// Measured (bf16): a piece of a 256 x 256 tile 1.6, of a 128 x 128 tile 0.55 alone on its CU with four buffers, 0.65 with two,
+// and 1.0 with two workgroups on a CU.  fp32 products are four times 128 x 128 x 32 in 1.8.
 static Plan gemm_plan(int kind, int32_t dtype, int64_t M, int64_t N, int64_t C) {
-    Plan p;
-    auto tiles = [&](int t, int64_t& tm, int64_t& tn) {
-        tm = (M + gemm_tile_m(t) - 1) / gemm_tile_m(t);
-        tn = (N + gemm_tile_n(t, kind) - 1) / gemm_tile_n(t, kind);
-    };
-    int64_t tm, tn;
-    tiles(TILE_256, tm, tn);
-    p.tile = TILE_256;
-    if (tm * tn < 192) {
-        p.tile = TILE_128;
-        tiles(TILE_128, tm, tn);
+    const bool f32 = dtype == HSTU_F32;
+    const int64_t bk = 128 / elem_bytes(dtype), pieces = (C + bk - 1) / bk;
+    Plan best = {};
+    double least = 1e300;
+    for (int tile = TILE_256; tile <= TILE_128_DEEP; tile++) {
+        const int64_t tm = (M + gemm_tile_m(tile) - 1) / gemm_tile_m(tile), tn = (N + gemm_tile_n(tile, kind) - 1) / gemm_tile_n(tile, kind);
+        for (int splits = 1; splits <= 64; splits *= 2) {
+            if (splits > 1 && (kind == GEMM_GATED || pieces < 2 * splits)) break;
+            const double wgs = (double)tm * tn * splits, share = (double)((pieces + splits - 1) / splits);
+            const bool pairs = tile == TILE_128 && wgs > 256;
+            const double piece = tile == TILE_256 ? (f32 ? 7.0 : 1.6) : f32 ? (pairs ? 3.6 : 1.8) : pairs ? 1.0 : tile == TILE_128 ? 0.65 : 0.55;
+            const double fixed = tile == TILE_256 ? 6.0 : pairs ? 4.0 : 3.0;
+            const double rounds = (double)(int64_t)((wgs + (pairs ? 511 : 255)) / (pairs ? 512 : 256));
+            double t = rounds * (fixed + share * piece);
+            if (splits > 1) t += 4.0 + (double)splits * M * N * 8 / 4.5e6;
+            if (t < least) {
+                least = t;
+                best.tile = tile;
+                best.tiles_m = (int)tm;
+                best.tiles_n = (int)tn;
+                best.splits = splits;
+            }
+        }
     }
-    p.tiles_m = (int)tm;
-    p.tiles_n = (int)tn;
-    p.splits = 1;
-    const int64_t bk = 128 / elem_bytes(dtype);
-    if (kind != GEMM_GATED) {
-        while (p.splits < 64 && tm * tn * p.splits * 2 <= 512 && C / (p.splits * 2) >= 512) p.splits *= 2;
-    }
-    const int64_t pieces = (C + bk - 1) / bk;
-    p.c_split = (pieces + p.splits - 1) / p.splits * bk;
-    p.splits = C > 0 ? (int)((C + p.c_split - 1) / p.c_split) : 1;
-    if (p.c_split == 0) p.c_split = bk;
-    return p;
+    best.c_split = (pieces + best.splits - 1) / best.splits * bk;
+    if (C > 0) best.splits = (int)((C + best.c_split - 1) / best.c_split);
+    else best.c_split = bk;
+    return best;
 }
 
 static int gemm_too_large(const Plan& p) {

@@ -92,8 +92,10 @@ __device__ __forceinline__ void swap_halves(unsigned& a, unsigned& b) {
     b = r[1];
 }
 
+template <int N> struct gm_const { static constexpr int value = N; };
+
 // ---- the kernel -----------------------------------------------------------------------------------------------------------
-template <typename T_, bool NRC_, bool MRC_, int BN_, int BM_, int WN_, int WM_, bool GATED_>
+template <typename T_, bool NRC_, bool MRC_, int BN_, int BM_, int WN_, int WM_, int STAGES_, bool GATED_>
 struct GemmShape {
     typedef T_ T;
     static constexpr bool NRC = NRC_, MRC = MRC_, GATED = GATED_;
@@ -102,9 +104,9 @@ struct GemmShape {
     static constexpr int WN = WN_, WM = WM_, NW = WN * WM, NT = 64 * NW;
     static constexpr int NB = BN / WN / 32, MB = BM / WM / 32;    // 32 x 32 blocks of a wave
     static constexpr int NI = BN / 8 / NW, MI = BM / 8 / NW;      // 1 KiB copies of a wave per piece and operand
-    static constexpr int N_BYTES = BN * 128, STAGE = (BN + BM) * 128;
+    static constexpr int N_BYTES = BN * 128, STAGE = (BN + BM) * 128, STAGES = STAGES_;
     static constexpr int STEPS = 4;                               // fragment steps per piece: 16 columns c of 16 bits, 8 of fp32
-    static_assert(!GATED || (NB == 2 && !NRC), "a gated wave holds one block of the gate and the matching one of the values");
+    static_assert(!GATED || (NB % 2 == 0 && !NRC), "a gated wave holds blocks of the gate and the matching ones of the values");
     static_assert(BN % (8 * NW) == 0 && BM % (8 * NW) == 0, "whole copies per wave");
 };
 
@@ -149,6 +151,10 @@ template <typename S, bool RC, int ROWS, int CNT> struct Stager {
     }
 };
 
+// The transposing LDS load.  The compiler has it wait for every copy into LDS that is under way, whatever part of LDS that
+// goes to, unless it knows more of the address: `restrict` is that knowledge (the kernel's own waits and barriers order the two).
+__device__ __forceinline__ gm_s16x4 read_tr(const char* __restrict__ at) { return __builtin_amdgcn_ds_read_tr16_b64_v4i16(GM_LDS(gm_s16x4, at)); }
+
 // fragment of 32 rows (block `blk` of the tile) and step s of the piece at `t`
 template <typename S, bool RC, int ROWS>
 __device__ __forceinline__ typename GM<typename S::T>::frag read_frag(const char* t, int blk, int s, int lane) {
@@ -161,8 +167,8 @@ __device__ __forceinline__ typename GM<typename S::T>::frag read_frag(const char
         const int rho = (lane >> 2) & 3;
         const int chunk = (4 * blk + 2 * (l32 >> 4) + ((lane & 3) >> 1)) ^ (4 * rho);
         const char* at = t + (16 * s + 8 * g + rho) * (ROWS * 2) + (chunk << 4) + 8 * (lane & 1);
-        const gm_s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(GM_LDS(gm_s16x4, at));
-        const gm_s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(GM_LDS(gm_s16x4, at + 4 * (ROWS * 2)));
+        const gm_s16x4 a = read_tr(at);
+        const gm_s16x4 b = read_tr(at + 4 * (ROWS * 2));
         const gm_s16x8 v = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
         return __builtin_bit_cast(frag, v);
     } else {
@@ -202,7 +208,7 @@ __global__ __launch_bounds__(S::NT) void hstu_gemm_kernel(const GemmArgs a) {
     typedef typename S::T T;
     typedef typename GM<T>::frag frag;
     constexpr int ES = S::ES, BK = S::BK, NB = S::NB, MB = S::MB;
-    __shared__ __attribute__((aligned(1024))) char gm_lds[2 * S::STAGE];
+    __shared__ __attribute__((aligned(1024))) char gm_lds[S::STAGES * S::STAGE];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 5, l32 = lane & 31;
     const int wn = w % S::WN, wm = w / S::WN;
@@ -241,41 +247,72 @@ __global__ __launch_bounds__(S::NT) void hstu_gemm_kernel(const GemmArgs a) {
             for (int r = 0; r < 16; r++) acc[i][j][r] = 0.f;
 
     const int64_t half = S::GATED ? (int64_t)a.N * a.n_ld * ES : 0;
+    // piece t into its place of the ring; behind the last one the copies address nothing, so that every turn issues as many
+    char* into = gm_lds;
+    int64_t c_left = c_len;
+    auto copy_in = [&]() __attribute__((always_inline)) {
+        const int left = (int)max(min(c_left, (int64_t)BK), (int64_t)0);
+        sn.issue(nb, into, w, left, half);
+        sm.issue(mb, into + S::N_BYTES, w, left, 0);
+        nb += n_step;
+        mb += m_step;
+        c_left -= BK;
+        into = into == gm_lds + (S::STAGES - 1) * S::STAGE ? gm_lds : into + S::STAGE;
+    };
+    // all but the newest `n` pieces' copies of this wave have landed
+    auto landed = [&](auto n) __attribute__((always_inline)) {
+        constexpr int left = decltype(n)::value * (S::NI + S::MI);
+        static_assert(left < 64, "the counter holds 63");
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(left) : "memory");
+    };
+    frag nf[2][NB], mf[2][MB];
+    auto read_step = [&](const char* cur, int s, frag (&n)[NB], frag (&m)[MB]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < NB; i++) {
+            const int blk = S::GATED ? (i / (NB / 2)) * (S::BN / 64) + wn * (NB / 2) + i % (NB / 2) : wn * NB + i;
+            n[i] = read_frag<S, S::NRC, S::BN>(cur, blk, s, lane);
+        }
+#pragma unroll
+        for (int j = 0; j < MB; j++) m[j] = read_frag<S, S::MRC, S::BM>(cur + S::N_BYTES, wm * MB + j, s, lane);
+    };
+    auto multiply = [&](const frag (&n)[NB], const frag (&m)[MB]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < NB; i++)
+#pragma unroll
+            for (int j = 0; j < MB; j++) acc[i][j] = GM<T>::mfma(n[i], m[j], acc[i][j]);
+    };
+    // The fragments of a step are read while the matrix cores work on the step before it, across the pieces too: the barrier
+    // that hands a piece over falls between the last reads of one and the first of the next, with a step's products queued.
     if (pieces > 0) {
-        const int left = (int)min(c_len, (int64_t)BK);
-        sn.issue(nb, gm_lds, w, left, half);
-        sm.issue(mb, gm_lds + S::N_BYTES, w, left, 0);
-    }
-    for (int t = 0; t < pieces; t++) {
-        // own copies landed, then everybody's; behind the barrier nobody reads the other buffer any more
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < S::STAGES; i++) copy_in();
+        landed(gm_const<S::STAGES - 1>());
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        char* cur = gm_lds + (t & 1) * S::STAGE;
-        if (t + 1 < pieces) {
-            char* nxt = gm_lds + ((t + 1) & 1) * S::STAGE;
-            nb += n_step;
-            mb += m_step;
-            const int left = (int)min(c_len - (int64_t)(t + 1) * BK, (int64_t)BK);
-            sn.issue(nb, nxt, w, left, half);
-            sm.issue(mb, nxt + S::N_BYTES, w, left, 0);
-        }
+        read_step(gm_lds, 0, nf[0], mf[0]);
+    }
+    const char* cur = gm_lds;
+    for (int t = 0; t < pieces; t++) {
+        const char* nxt = cur == gm_lds + (S::STAGES - 1) * S::STAGE ? gm_lds : cur + S::STAGE;
 #pragma unroll
         for (int s = 0; s < S::STEPS; s++) {
-            frag nf[NB], mf[MB];
-#pragma unroll
-            for (int i = 0; i < NB; i++) {
-                const int blk = S::GATED ? i * (S::BN / 64) + wn : wn * NB + i;
-                nf[i] = read_frag<S, S::NRC, S::BN>(cur, blk, s, lane);
+            if (s + 1 < S::STEPS) read_step(cur, s + 1, nf[(s + 1) & 1], mf[(s + 1) & 1]);
+            else if (t + 1 < pieces) {
+                // own reads of this piece and own copies of the next have landed; behind the barrier everybody's have, and
+                // this piece's place is free
+                landed(gm_const<S::STAGES - 2>());
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+                copy_in();
+                read_step(nxt, 0, nf[0], mf[0]);
             }
-#pragma unroll
-            for (int j = 0; j < MB; j++) mf[j] = read_frag<S, S::MRC, S::BM>(cur + S::N_BYTES, wm * MB + j, s, lane);
-#pragma unroll
-            for (int i = 0; i < NB; i++)
-#pragma unroll
-                for (int j = 0; j < MB; j++) acc[i][j] = GM<T>::mfma(nf[i], mf[j], acc[i][j]);
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(nf[s & 1], mf[s & 1]);
+            __builtin_amdgcn_sched_barrier(0);
         }
+        cur = nxt;
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // copies of nothing may still be under way
 
     // accumulator register r of block (i, j): row m = 32 j + l32, n = 32 i + 8 (r / 4) + 4 g + r % 4 of the wave's tile
     if constexpr (!S::GATED) {
@@ -294,7 +331,9 @@ __global__ __launch_bounds__(S::NT) void hstu_gemm_kernel(const GemmArgs a) {
             }
         }
     } else {
-        const int n = n0 + wn * 32;
+#pragma unroll
+        for (int gb = 0; gb < NB / 2; gb++) {
+        const int n = n0 + (wn * (NB / 2) + gb) * 32;
         float bg[16], bu[16];
 #pragma unroll
         for (int r = 0; r < 16; r++) {
@@ -318,8 +357,8 @@ __global__ __launch_bounds__(S::NT) void hstu_gemm_kernel(const GemmArgs a) {
             float zg[16], zu[16], h[16];
 #pragma unroll
             for (int r = 0; r < 16; r++) {
-                zg[r] = acc[0][j][r] + bg[r];
-                zu[r] = acc[1][j][r] + bu[r];
+                zg[r] = acc[gb][j][r] + bg[r];
+                zu[r] = acc[NB / 2 + gb][j][r] + bu[r];
                 h[r] = act_of(zg[r], a.act) * zu[r];
             }
             store_block<T>(reinterpret_cast<T*>(a.out) + m * a.N + n, h, g, left);
@@ -355,12 +394,15 @@ __global__ __launch_bounds__(S::NT) void hstu_gemm_kernel(const GemmArgs a) {
                 }
             }
         }
+        }
     }
 }
 
 // kinds of products, and the launchers (one translation unit per element type)
 enum GemmKind : int { GEMM_GATED = 0 /* KC x KC, gated epilogue */, GEMM_DX = 1 /* n side RC, m side KC */, GEMM_DW = 2 /* both RC */ };
-enum GemmTile : int { TILE_256 = 0, TILE_128 = 1 };
+// 256 x 256 outputs by eight waves (one workgroup per CU); 128 x 128 by four, with two buffers (two workgroups per CU) or four (one,
+// whose copies run three pieces ahead)
+enum GemmTile : int { TILE_256 = 0, TILE_128 = 1, TILE_128_DEEP = 2 };
 constexpr int gemm_tile_m(int tile) { return tile == TILE_256 ? 256 : 128; }
 constexpr int gemm_tile_n(int tile, int kind) { return (tile == TILE_256 ? 256 : 128) / (kind == GEMM_GATED ? 2 : 1); }
 hipError_t launch_gemm_bf16(const GemmArgs& a, int kind, int tile, hipStream_t st);
@@ -372,10 +414,13 @@ template <typename T> hipError_t launch_gemm_t(const GemmArgs& a, int kind, int 
 #define GM_GO(NRC, MRC, GATED)                                                                                                  \
     do {                                                                                                                        \
         if (tile == TILE_256) {                                                                                                 \
-            typedef GemmShape<T, NRC, MRC, 256, 256, 4, 2, GATED> S;                                                            \
+            typedef GemmShape<T, NRC, MRC, 256, 256, 4, 2, 2, GATED> S;                                                            \
+            hipLaunchKernelGGL((hstu_gemm_kernel<S>), grid, dim3(S::NT), 0, st, a);                                             \
+        } else if (tile == TILE_128) {                                                                                          \
+            typedef GemmShape<T, NRC, MRC, 128, 128, 2, 2, 2, GATED> S;                                                         \
             hipLaunchKernelGGL((hstu_gemm_kernel<S>), grid, dim3(S::NT), 0, st, a);                                             \
         } else {                                                                                                                \
-            typedef GemmShape<T, NRC, MRC, 128, 128, 2, 2, GATED> S;                                                            \
+            typedef GemmShape<T, NRC, MRC, 128, 128, 2, 2, 4, GATED> S;                                                         \
             hipLaunchKernelGGL((hstu_gemm_kernel<S>), grid, dim3(S::NT), 0, st, a);                                             \
         }                                                                                                                       \
     } while (0)
