@@ -7,7 +7,7 @@
 // dz is rounded to the I/O type between the two: the products run on the 16-bit matrix cores, and the rounding (2^-9 relative
 // per element, independent) averages out over sums of 2 f and of m terms.
 #include "hstu_ffn_common.h"
-#include "hstu_gemm.h"
+#include "hstu_gated_rows.h"
 
 namespace hstu {
 
@@ -143,7 +143,7 @@ static hipError_t launch_gemm(int32_t dtype, const GemmArgs& a, int kind, int ti
     return launch_gemm_bf16(a, kind, tile, st);
 }
 
-struct Plan { int tile, splits, tiles_n, tiles_m; int64_t c_split; };
+struct Plan { int tile, splits, tiles_n, tiles_m; int64_t c_split; double us; };
 
 // Tiles and shares of the contraction: the cheapest by a model of the launch, in microseconds.  A workgroup takes a start and an
 // end (`fixed`) and `piece` for each piece of its share; workgroups come in rounds of what the chip holds at a time; shares
@@ -167,7 +167,7 @@ static Plan gemm_plan(int kind, int32_t dtype, int64_t M, int64_t N, int64_t C) 
             double t = rounds * (fixed + share * piece);
             if (splits > 1) t += 4.0 + (double)splits * M * N * 8 / 4.5e6;
             if (t < least) {
-                least = t;
+                least = best.us = t;
                 best.tile = tile;
                 best.tiles_m = (int)tm;
                 best.tiles_n = (int)tn;
@@ -213,10 +213,20 @@ static int gated_check_sizes(int32_t dtype, int32_t act, int32_t keep, int64_t m
     return HSTU_OK;
 }
 
+// Few rows go to the kernel that reads W straight into fragments, as long as its workgroups' reading of x, f / 16 times, costs
+// less than tiles of 128 rows that are mostly empty.  Measured (bf16, k 1024): at f 4096, 4.3 us for one row and 8.1 for 64 against
+// 12.2 and 12.4 in tiles; at f 16384, 12.0 and 24.9 against 13.9 and 14.6, so that tiles take over at about 16 rows there.
+static bool few_rows(const hstu_gated_params* p) {
+    if (p->m > ROWS_MAX_M) return false;
+    const double e = elem_bytes(p->dtype), w = 2.0 * p->f * p->k * e, x = (p->f / 16.0) * p->m * p->k * e;
+    return 2.2 + w / 7e6 + x / 9e6 <= gemm_plan(GEMM_GATED, p->dtype, p->m, p->f, p->k).us + 2.5;
+}
+
 struct GatedLayout { uint64_t x, w, bytes; bool pad_x, pad_w; };
 static GatedLayout gated_layout(const hstu_gated_params* p) {
     GatedLayout l;
     const uint64_t e = elem_bytes(p->dtype), ld = padded(p->k, p->dtype);
+    if (few_rows(p)) { l = {}; return l; }
     l.pad_x = p->m > 0 && needs_pad(p->x, p->m > 1 ? p->x_stride : ld, p->k, p->dtype);
     l.pad_w = p->m > 0 && needs_pad(p->weight, p->k, p->k, p->dtype);
     l.x = 0;
@@ -344,10 +354,19 @@ extern "C" int hstu_hip_gated_linear(const hstu_gated_params* p, void* workspace
     const GatedLayout l = gated_layout(p);
     rc = check_workspace(workspace, workspace_bytes, l.bytes);
     if (rc != HSTU_OK) return rc;
+    hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    if (few_rows(p)) {
+        RowsArgs a = {};
+        a.x = p->x; a.weight = p->weight; a.bias = p->bias; a.out = p->out; a.z = p->z; a.z_exp = p->z_exponents;
+        a.x_stride = p->x_stride;
+        a.m = (int32_t)p->m; a.k = p->k; a.f = p->f; a.bias_f32 = p->bias_dtype == HSTU_F32; a.act = p->act; a.keep = p->keep;
+        const hipError_t e = p->dtype == HSTU_F32 ? launch_gated_rows_f32(a, st) : p->dtype == HSTU_F16 ? launch_gated_rows_f16(a, st) : launch_gated_rows_bf16(a, st);
+        if (e != hipSuccess) return fail(HSTU_ERR_LAUNCH, "kernel launch failed: %s", hipGetErrorString(e));
+        return HSTU_OK;
+    }
     const Plan pl = gemm_plan(GEMM_GATED, p->dtype, p->m, p->f, p->k);
     rc = gemm_too_large(pl);
     if (rc != HSTU_OK) return rc;
-    hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     char* ws = reinterpret_cast<char*>(workspace);
     const int64_t ld = padded(p->k, p->dtype);
     hipError_t e = hipSuccess;
