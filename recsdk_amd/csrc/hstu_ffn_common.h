@@ -11,37 +11,92 @@ typedef __attribute__((ext_vector_type(2))) unsigned int ffn_u2;
 typedef ffn_u4 __attribute__((aligned(1))) ffn_u4_any;
 typedef ffn_u2 __attribute__((aligned(1))) ffn_u2_any;
 
-// the first min(n, 8) of 8 consecutive elements, zero behind them.  The rows are streamed: nontemporal
-template <typename T> __device__ __forceinline__ void load8_any(const T* p, int n, float* v) {
+typedef unsigned int __attribute__((aligned(1))) ffn_u1_any;
+typedef unsigned short __attribute__((aligned(1))) ffn_h1_any;
+
+// the first min(n, 8) of 8 consecutive elements, zero behind them: as they lie in memory, so that a row can be under way while
+// another is worked on, and as floats.  The rows are streamed: nontemporal.  The end of a row goes in pieces of four, two and
+// one elements, in registers
+template <typename T> struct Raw8 { ffn_u4 q[8 * sizeof(T) / 16]; };
+template <typename T> __device__ __forceinline__ Raw8<T> load8_raw(const T* p, int n) {
+    Raw8<T> r;
     if (n >= 8) {
-        T t[8];
 #pragma unroll
-        for (int q = 0; q < (int)(8 * sizeof(T) / 16); q++) {
-            const ffn_u4 x = __builtin_nontemporal_load(reinterpret_cast<const ffn_u4_any*>(p) + q);
-            __builtin_memcpy(reinterpret_cast<char*>(t) + 16 * q, &x, 16);
-        }
-#pragma unroll
-        for (int k = 0; k < 8; k++) v[k] = to_float(t[k]);
-    } else {
-#pragma unroll
-        for (int k = 0; k < 8; k++) v[k] = k < n ? to_float(p[k]) : 0.f;
+        for (int q = 0; q < (int)(8 * sizeof(T) / 16); q++) r.q[q] = __builtin_nontemporal_load(reinterpret_cast<const ffn_u4_any*>(p) + q);
+        return r;
     }
+#pragma unroll
+    for (int q = 0; q < (int)(8 * sizeof(T) / 16); q++) r.q[q] = ffn_u4{0u, 0u, 0u, 0u};
+    if (n <= 0) return r;
+    const bool four = n & 4, two = n & 2;
+    if constexpr (sizeof(T) == 2) {
+        unsigned w0 = 0, w1 = 0, w2 = 0, w3 = 0;
+        if (four) {
+            const ffn_u2 x = *reinterpret_cast<const ffn_u2_any*>(p);
+            w0 = x[0];
+            w1 = x[1];
+        }
+        if (two) {
+            const unsigned x = *reinterpret_cast<const ffn_u1_any*>(p + (four ? 4 : 0));
+            w0 = four ? w0 : x;
+            w2 = four ? x : 0u;
+        }
+        if (n & 1) {
+            const unsigned x = *reinterpret_cast<const ffn_h1_any*>(p + (four ? 4 : 0) + (two ? 2 : 0));
+            w0 = !four && !two ? x : w0;
+            w1 = !four && two ? x : w1;
+            w2 = four && !two ? x : w2;
+            w3 = four && two ? x : w3;
+        }
+        r.q[0] = ffn_u4{w0, w1, w2, w3};
+    } else {
+        ffn_u4 lo = {0u, 0u, 0u, 0u}, hi = lo;
+        if (four) lo = *reinterpret_cast<const ffn_u4_any*>(p);
+        if (two) {
+            const ffn_u2 x = *reinterpret_cast<const ffn_u2_any*>(p + (four ? 4 : 0));
+            if (four) { hi[0] = x[0]; hi[1] = x[1]; }
+            else { lo[0] = x[0]; lo[1] = x[1]; }
+        }
+        if (n & 1) {
+            const unsigned x = *reinterpret_cast<const ffn_u1_any*>(p + (four ? 4 : 0) + (two ? 2 : 0));
+            if (four) { hi[0] = two ? hi[0] : x; hi[2] = two ? x : 0u; }
+            else { lo[0] = two ? lo[0] : x; lo[2] = two ? x : 0u; }
+        }
+        r.q[0] = lo;
+        r.q[sizeof(T) == 4 ? 1 : 0] = hi;
+    }
+    return r;
 }
+template <typename T> __device__ __forceinline__ void to_floats(const Raw8<T>& r, float* v) {
+    T t[8];
+    __builtin_memcpy(t, &r, sizeof(r));
+#pragma unroll
+    for (int k = 0; k < 8; k++) v[k] = to_float(t[k]);
+}
+template <typename T> __device__ __forceinline__ void load8_any(const T* p, int n, float* v) { to_floats(load8_raw(p, n), v); }
 template <typename T> __device__ __forceinline__ void store8_any(T* p, int n, const float* v) {
     T t[8];
 #pragma unroll
     for (int k = 0; k < 8; k++) t[k] = from_float<T>(v[k]);
+    Raw8<T> r;
+    __builtin_memcpy(&r, t, sizeof(r));
     if (n >= 8) {
 #pragma unroll
-        for (int q = 0; q < (int)(8 * sizeof(T) / 16); q++) {
-            ffn_u4 x;
-            __builtin_memcpy(&x, reinterpret_cast<char*>(t) + 16 * q, 16);
-            __builtin_nontemporal_store(x, reinterpret_cast<ffn_u4_any*>(p) + q);
-        }
+        for (int q = 0; q < (int)(8 * sizeof(T) / 16); q++) __builtin_nontemporal_store(r.q[q], reinterpret_cast<ffn_u4_any*>(p) + q);
+        return;
+    }
+    if (n <= 0) return;
+    const bool four = n & 4, two = n & 2;
+    if constexpr (sizeof(T) == 2) {
+        const ffn_u4 w = r.q[0];
+        if (four) *reinterpret_cast<ffn_u2_any*>(p) = ffn_u2{w[0], w[1]};
+        if (two) *reinterpret_cast<ffn_u1_any*>(p + (four ? 4 : 0)) = four ? w[2] : w[0];
+        if (n & 1) *reinterpret_cast<ffn_h1_any*>(p + (four ? 4 : 0) + (two ? 2 : 0)) = (unsigned short)(four ? (two ? w[3] : w[2]) : (two ? w[1] : w[0]));
     } else {
-#pragma unroll
-        for (int k = 0; k < 8; k++)
-            if (k < n) p[k] = t[k];
+        const ffn_u4 lo = r.q[0], hi = r.q[sizeof(T) == 4 ? 1 : 0];
+        if (four) *reinterpret_cast<ffn_u4_any*>(p) = lo;
+        if (two) *reinterpret_cast<ffn_u2_any*>(p + (four ? 4 : 0)) = four ? ffn_u2{hi[0], hi[1]} : ffn_u2{lo[0], lo[1]};
+        if (n & 1) *reinterpret_cast<ffn_u1_any*>(p + (four ? 4 : 0) + (two ? 2 : 0)) = four ? (two ? hi[2] : hi[0]) : (two ? lo[2] : lo[0]);
     }
 }
 

@@ -10,16 +10,34 @@
 
 namespace hstu {
 
-constexpr int LN_MAX_WGS = 1024;   // workgroups of the backward = rows of its partial-sum table
+// sum over groups of N neighbouring lanes, in every lane.  Register moves between lanes instead of LDS permutes: within a quad, then
+// mirrored in 8 and 16 lanes (whose halves hold equal sums by then), then the two instructions that exchange rows of 16 and halves
+template <int CTRL> __device__ __forceinline__ float ln_moved(float x) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
+}
+template <int N> __device__ __forceinline__ float ln_lanes_sum(float x) {
+    x += ln_moved<0xB1>(x);                          // quad_perm 1 0 3 2
+    x += ln_moved<0x4E>(x);                          // quad_perm 2 3 0 1
+    if constexpr (N >= 8) x += ln_moved<0x141>(x);   // mirror of 8
+    if constexpr (N >= 16) x += ln_moved<0x140>(x);  // mirror of 16
+    if constexpr (N >= 32) {
+        const unsigned u = __builtin_bit_cast(unsigned, x);
+        const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+        x = __builtin_bit_cast(float, (unsigned)r[0]) + __builtin_bit_cast(float, (unsigned)r[1]);
+    }
+    if constexpr (N >= 64) {
+        const unsigned u = __builtin_bit_cast(unsigned, x);
+        const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+        x = __builtin_bit_cast(float, (unsigned)r[0]) + __builtin_bit_cast(float, (unsigned)r[1]);
+    }
+    return x;
+}
 
 // sums of a and b over the LPR lanes of a row; `slot` (0 / 1, alternating) keeps a workgroup-wide sum from meeting the next
 // one in LDS
 template <int LPR> __device__ __forceinline__ void ln_sum(float& a, float& b, float* red, int slot) {
-#pragma unroll
-    for (int o = (LPR < 64 ? LPR : 64) / 2; o > 0; o >>= 1) {
-        a += __shfl_xor(a, o, 64);
-        b += __shfl_xor(b, o, 64);
-    }
+    a = ln_lanes_sum<(LPR < 64 ? LPR : 64)>(a);
+    b = ln_lanes_sum<(LPR < 64 ? LPR : 64)>(b);
     if constexpr (LPR > 64) {
         constexpr int W = LPR / 64;
         float* at = red + slot * 2 * W;
@@ -61,14 +79,22 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void hstu_layer_norm_fwd_ker
         ln_param<T>(p.weight, f32, c, p.cols - c, 1.f, w[q]);
         ln_param<T>(p.bias, f32, c, p.cols - c, 0.f, b[q]);
     }
-    for (int64_t row = (int64_t)blockIdx.x * RPW + threadIdx.x / LPR; row < p.rows; row += (int64_t)gridDim.x * RPW) {
-        const T* x = reinterpret_cast<const T*>(p.x) + row * p.x_stride;
-        float v[NP][8], s = 0.f, none = 0.f;
+    const int64_t step = (int64_t)gridDim.x * RPW;
+    int64_t row = (int64_t)blockIdx.x * RPW + threadIdx.x / LPR;
+    Raw8<T> next[NP];   // the row after the one that is worked on is under way
+    auto fetch = [&](int64_t r) __attribute__((always_inline)) {
 #pragma unroll
         for (int q = 0; q < NP; q++) {
             const int c = (q * LPR + l) * 8;
-            load8_any(x + c, p.cols - c, v[q]);
+            next[q] = load8_raw(reinterpret_cast<const T*>(p.x) + r * p.x_stride + c, p.cols - c);
         }
+    };
+    if (row < p.rows) fetch(row);
+    for (; row < p.rows; row += step) {
+        float v[NP][8], s = 0.f, none = 0.f;
+#pragma unroll
+        for (int q = 0; q < NP; q++) to_floats(next[q], v[q]);
+        if (row + step < p.rows) fetch(row + step);
 #pragma unroll
         for (int q = 0; q < NP; q++)
 #pragma unroll
@@ -120,17 +146,32 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void hstu_layer_norm_bwd_ker
         for (int k = 0; k < 8; k++) gw[q][k] = gb[q][k] = 0.f;
     }
     int slot = 0;
-    for (int64_t row = (int64_t)blockIdx.x * RPW + threadIdx.x / LPR; row < p.rows; row += (int64_t)gridDim.x * RPW) {
-        const T* x = reinterpret_cast<const T*>(p.x) + row * p.x_stride;
-        const T* dy = reinterpret_cast<const T*>(p.d_y) + row * p.dy_stride;
-        const float mean = p.mean[row], rstd = p.rstd[row];
-        float xh[NP][8], g[NP][8];
+    const int64_t step = (int64_t)gridDim.x * RPW;
+    int64_t row = (int64_t)blockIdx.x * RPW + threadIdx.x / LPR;
+    constexpr bool AHEAD = LPR < 1024;   // (a lane of a 1024-wide workgroup has 128 registers: its row is fetched when it is due)
+    Raw8<T> next_x[NP], next_g[NP];      // the row after the one that is worked on is under way
+    float next_mean = 0.f, next_rstd = 0.f;
+    auto fetch = [&](int64_t r) __attribute__((always_inline)) {
+        next_mean = p.mean[r];
+        next_rstd = p.rstd[r];
 #pragma unroll
         for (int q = 0; q < NP; q++) {
             const int c = (q * LPR + l) * 8;
-            load8_any(x + c, p.cols - c, xh[q]);
-            load8_any(dy + c, p.cols - c, g[q]);
+            next_x[q] = load8_raw(reinterpret_cast<const T*>(p.x) + r * p.x_stride + c, p.cols - c);
+            next_g[q] = load8_raw(reinterpret_cast<const T*>(p.d_y) + r * p.dy_stride + c, p.cols - c);
         }
+    };
+    if (AHEAD && row < p.rows) fetch(row);
+    for (; row < p.rows; row += step) {
+        if (!AHEAD) fetch(row);
+        const float mean = next_mean, rstd = next_rstd;
+        float xh[NP][8], g[NP][8];
+#pragma unroll
+        for (int q = 0; q < NP; q++) {
+            to_floats(next_x[q], xh[q]);
+            to_floats(next_g[q], g[q]);
+        }
+        if (AHEAD && row + step < p.rows) fetch(row + step);
         float s1 = 0.f, s2 = 0.f;
 #pragma unroll
         for (int q = 0; q < NP; q++)
@@ -201,7 +242,7 @@ template <typename T> __global__ __launch_bounds__(1024) void hstu_colsum_kernel
     const int64_t width = 2 * (int64_t)half, c = (int64_t)blockIdx.x * 32 + tx;
     float s = 0.f;
     if (c < width)
-#pragma unroll 4
+#pragma unroll 8
         for (int r = ty; r < rows; r += 32) s += partial[r * width + c];
     part[ty][tx] = s;
     __syncthreads();
@@ -222,17 +263,26 @@ hipError_t launch_colsum(const float* partial, int rows, int half, void* out0, v
     return hipGetLastError();
 }
 
-// lanes per row and pieces per lane: the smallest pair that holds the row
+// lanes per row and pieces per lane: the smallest pair that holds the row.  (32, 2) and not (64, 1) up to 512 columns: two rows a wave
+// (262144 rows bf16: 512 columns 110 -> 104 us forward, 257 columns 102 -> 87 and 191 -> 161 us backward)
 struct LnShape { int lpr, np; };
 static LnShape ln_shape(int cols) {
-    static const LnShape s[] = {{8, 1}, {16, 1}, {32, 1}, {64, 1}, {64, 2}, {64, 4}, {256, 2}, {512, 2}, {1024, 2}};
+    static const LnShape s[] = {{8, 1}, {16, 1}, {32, 1}, {32, 2}, {64, 2}, {64, 4}, {256, 2}, {512, 2}, {1024, 2}};
     for (const LnShape& x : s)
         if (x.lpr * x.np * 8 >= cols) return x;
     return s[8];
 }
 static int ln_rows_per_wg(const LnShape& s) { return s.lpr > 256 ? 1 : 256 / s.lpr; }
-static unsigned ln_grid(int64_t rows, const LnShape& s, int64_t most) {
+// Workgroups that walk down the rows with the next one under way.  Forward: up to 2048 (262144 x 128 fp16: 38 us with a workgroup
+// for every 16 rows, 28 with 2048; 30000 x 2048 bf16: 80 and 56, since a row's weight and bias are loaded once a lane).
+static unsigned ln_fwd_grid(int64_t rows, const LnShape& s) {
     const int64_t n = (rows + ln_rows_per_wg(s) - 1) / ln_rows_per_wg(s);
+    return (unsigned)(n < 1 ? 1 : n > 2048 ? 2048 : n);
+}
+// Backward: each one is a row of the partial-sum table too, so no more than fill the chip and two rows a lane at least
+// (262144 x 512 bf16: 148 us with 1024, 137 with 768, 214 with 256; 16384 x 8192: 182, 170 and 146)
+static unsigned ln_bwd_grid(int64_t rows, const LnShape& s) {
+    const int64_t most = s.lpr > 256 ? 256 : s.np > 1 ? 512 : 768, per = 2 * ln_rows_per_wg(s), n = (rows + per - 1) / per;
     return (unsigned)(n < 1 ? 1 : n > most ? most : n);
 }
 
@@ -258,7 +308,7 @@ using namespace hstu;
             case 8 * 8 + 1: hipLaunchKernelGGL((KERNEL<T, 8, 1>), grid, nt, 0, st, __VA_ARGS__); break;                   \
             case 16 * 8 + 1: hipLaunchKernelGGL((KERNEL<T, 16, 1>), grid, nt, 0, st, __VA_ARGS__); break;                 \
             case 32 * 8 + 1: hipLaunchKernelGGL((KERNEL<T, 32, 1>), grid, nt, 0, st, __VA_ARGS__); break;                 \
-            case 64 * 8 + 1: hipLaunchKernelGGL((KERNEL<T, 64, 1>), grid, nt, 0, st, __VA_ARGS__); break;                 \
+            case 32 * 8 + 2: hipLaunchKernelGGL((KERNEL<T, 32, 2>), grid, nt, 0, st, __VA_ARGS__); break;                 \
             case 64 * 8 + 2: hipLaunchKernelGGL((KERNEL<T, 64, 2>), grid, nt, 0, st, __VA_ARGS__); break;                 \
             case 64 * 8 + 4: hipLaunchKernelGGL((KERNEL<T, 64, 4>), grid, nt, 0, st, __VA_ARGS__); break;                 \
             case 256 * 8 + 2: hipLaunchKernelGGL((KERNEL<T, 256, 2>), grid, nt, 0, st, __VA_ARGS__); break;               \
@@ -288,7 +338,7 @@ extern "C" int hstu_hip_layer_norm(const hstu_layer_norm_params* p, void* stream
         return fail(HSTU_ERR_UNSUPPORTED, "x, weight, bias and y must be aligned to their element types");
     const LnShape s = ln_shape(p->cols);
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    LN_DISPATCH(p->dtype, hstu_layer_norm_fwd_kernel, s, dim3(ln_grid(p->rows, s, 16384)), st, *p);
+    LN_DISPATCH(p->dtype, hstu_layer_norm_fwd_kernel, s, dim3(ln_fwd_grid(p->rows, s)), st, *p);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return fail(HSTU_ERR_LAUNCH, "kernel launch failed: %s", hipGetErrorString(e));
     return HSTU_OK;
@@ -312,7 +362,7 @@ static int ln_bwd_validate(const hstu_layer_norm_bwd_params* p) {
 
 static uint64_t ln_bwd_bytes(const hstu_layer_norm_bwd_params* p) {
     if (!p->d_weight && !p->d_bias) return 0;
-    return (uint64_t)ln_grid(p->rows, ln_shape(p->cols), LN_MAX_WGS) * 2 * p->cols * sizeof(float);
+    return (uint64_t)ln_bwd_grid(p->rows, ln_shape(p->cols)) * 2 * p->cols * sizeof(float);
 }
 
 extern "C" int hstu_hip_layer_norm_backward_get_workspace_size(const hstu_layer_norm_bwd_params* p, uint64_t* bytes) {
@@ -333,7 +383,7 @@ extern "C" int hstu_hip_layer_norm_backward(const hstu_layer_norm_bwd_params* p,
     if (!p->d_x && !p->d_weight && !p->d_bias) return HSTU_OK;
     if (p->rows == 0 && !need) return HSTU_OK;
     const LnShape s = ln_shape(p->cols);
-    const unsigned grid = ln_grid(p->rows, s, LN_MAX_WGS);
+    const unsigned grid = ln_bwd_grid(p->rows, s);
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     float* partial = need ? reinterpret_cast<float*>(workspace) : nullptr;
     // without rows the workgroups write zero sums
