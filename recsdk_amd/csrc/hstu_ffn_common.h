@@ -112,7 +112,7 @@ __device__ __forceinline__ void act_and_grad(float z, int act, float& a, float& 
     if (act == HSTU_ACT_SILU) {
         const float s = sigmoid_of(z);
         a = z * s;
-        d = s * (1.0f + z * (1.0f - s));
+        d = __builtin_fmaf(a, 1.0f - s, s);   // s (1 + z (1 - s))
     } else {
         const float phi = 0.5f * erfcf(-0.70710678f * z);
         a = z * phi;
@@ -145,19 +145,24 @@ __device__ __forceinline__ unsigned pack8_codes(float a, float b, float c, float
     return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
 }
 
-// the values of the first min(n, 8) of 8 consecutive codes of one group, brought into [-top, top]; zero behind them
-__device__ __forceinline__ void unpack8_any(const uint8_t* p, int n, int byte, float top, float* v) {
-    ffn_u2 q = {0u, 0u};
-    if (n >= 8) q = __builtin_nontemporal_load(reinterpret_cast<const ffn_u2_any*>(p));
-    else {
+// the first min(n, 8) of 8 consecutive codes of one group with its exponent byte, and the values they stand for, brought into
+// [-top, top] (zero codes behind them)
+struct Codes8 { ffn_u2 q; int byte; };
+__device__ __forceinline__ Codes8 codes8_raw(const uint8_t* p, int n, int byte) {
+    Codes8 r = {{0u, 0u}, byte};
+    if (n >= 8) r.q = __builtin_nontemporal_load(reinterpret_cast<const ffn_u2_any*>(p));
+    else if (n > 0) {
 #pragma unroll
         for (int k = 0; k < 8; k++)
-            if (k < n) q[k >> 2] |= (unsigned)p[k] << (8 * (k & 3));
+            if (k < n) r.q[k >> 2] |= (unsigned)p[k] << (8 * (k & 3));
     }
-    const float scale = pack8_scale(byte);
+    return r;
+}
+__device__ __forceinline__ void code_values(const Codes8& c, float top, float* v) {
+    const float scale = pack8_scale(c.byte);
 #pragma unroll
     for (int h = 0; h < 2; h++) {
-        const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)q[h], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)q[h], true);
+        const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)c.q[h], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)c.q[h], true);
         const float w[4] = {lo[0], lo[1], hi[0], hi[1]};
 #pragma unroll
         for (int k = 0; k < 4; k++) {

@@ -14,16 +14,18 @@ namespace hstu {
 // ---- rows to 16-byte boundaries ------------------------------------------------------------------------------------------
 // The product's copies move aligned 16-byte pieces.  An operand whose rows do not start on such boundaries, or end inside a
 // piece, is first copied to rows of `ld` elements, zeros behind each row.
+struct PadArgs { const void* src[2]; void* dst[2]; int64_t stride[2], rows[2]; int64_t ld; int32_t cols; };   // up to two operands, one launch
 template <typename T>
-__global__ __launch_bounds__(256) void hstu_pad_rows_kernel(const T* src, int64_t stride, int64_t rows, int cols, T* dst, int64_t ld) {
-    const int per_row = (int)(ld / 8 + (ld % 8 ? 1 : 0));   // pieces of 8 elements
-    const int64_t n = rows * per_row;
+__global__ __launch_bounds__(256) void hstu_pad_rows_kernel(const PadArgs a) {
+    const int per_row = (int)((a.ld + 7) / 8);   // pieces of 8 elements
+    const int64_t first = a.rows[0] * per_row, n = first + a.rows[1] * per_row;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        const int64_t r = i / per_row;
-        const int c = (int)(i - r * per_row) * 8;
+        const int which = i >= first;
+        const int64_t j = which ? i - first : i, r = j / per_row;
+        const int c = (int)(j - r * per_row) * 8;
         float v[8];
-        load8_any(src + r * stride + (cols - c > 0 ? c : 0), cols - c, v);
-        store8_any(dst + r * ld + c, (int)(ld - c), v);
+        load8_any(reinterpret_cast<const T*>(a.src[which]) + r * a.stride[which] + (a.cols - c > 0 ? c : 0), a.cols - c, v);
+        store8_any(reinterpret_cast<T*>(a.dst[which]) + r * a.ld + c, (int)(a.ld - c), v);
     }
 }
 
@@ -60,8 +62,8 @@ __global__ __launch_bounds__(256) void hstu_gated_dz_kernel(const DzArgs a) {
             if (a.keep == HSTU_KEEP_8BIT) {
                 const uint8_t* z = reinterpret_cast<const uint8_t*>(a.z) + r * 2 * a.f + c;
                 const uint8_t* e = a.z_exp + r * 2 * groups + c / HSTU_PACK8_GROUP;
-                unpack8_any(z, n, e[0], largest_finite<float>(), zg);
-                unpack8_any(z + a.f, n, e[groups], largest_finite<float>(), zu);
+                code_values(codes8_raw(z, n, e[0]), largest_finite<float>(), zg);
+                code_values(codes8_raw(z + a.f, n, e[groups]), largest_finite<float>(), zu);
             } else {
                 const T* z = reinterpret_cast<const T*>(a.z) + r * 2 * a.f + c;
                 load8_any(z, n, zg);
@@ -191,13 +193,20 @@ static void fill(GemmArgs& a, const Plan& pl, int64_t M, int64_t N, int64_t C) {
     a.c_split = pl.c_split; a.splits = pl.splits; a.tiles_m = pl.tiles_m; a.tiles_n = pl.tiles_n;
 }
 
-static hipError_t launch_pad(int32_t dtype, const void* src, int64_t stride, int64_t rows, int cols, void* dst, int64_t ld, hipStream_t st) {
+// x (where `x` is given a place) and weight (likewise) to rows of `ld` elements
+static hipError_t launch_pad(int32_t dtype, const void* x, int64_t x_stride, int64_t m, void* x_to, const void* w, int64_t f2, void* w_to, int k, int64_t ld, hipStream_t st) {
+    PadArgs a = {};
+    a.ld = ld;
+    a.cols = k;
+    a.src[0] = x; a.stride[0] = x_stride; a.dst[0] = x_to; a.rows[0] = x_to ? m : 0;
+    a.src[1] = w; a.stride[1] = k; a.dst[1] = w_to; a.rows[1] = w_to ? f2 : 0;
+    const int64_t rows = a.rows[0] + a.rows[1];
     if (rows == 0) return hipSuccess;
     const int64_t want = (rows * ((ld + 7) / 8) + 255) / 256;
     const dim3 grid((unsigned)(want > 4096 ? 4096 : want));
-    if (dtype == HSTU_F32) hipLaunchKernelGGL(hstu_pad_rows_kernel<float>, grid, dim3(256), 0, st, (const float*)src, stride, rows, cols, (float*)dst, ld);
-    else if (dtype == HSTU_F16) hipLaunchKernelGGL(hstu_pad_rows_kernel<_Float16>, grid, dim3(256), 0, st, (const _Float16*)src, stride, rows, cols, (_Float16*)dst, ld);
-    else hipLaunchKernelGGL(hstu_pad_rows_kernel<__bf16>, grid, dim3(256), 0, st, (const __bf16*)src, stride, rows, cols, (__bf16*)dst, ld);
+    if (dtype == HSTU_F32) hipLaunchKernelGGL(hstu_pad_rows_kernel<float>, grid, dim3(256), 0, st, a);
+    else if (dtype == HSTU_F16) hipLaunchKernelGGL(hstu_pad_rows_kernel<_Float16>, grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(hstu_pad_rows_kernel<__bf16>, grid, dim3(256), 0, st, a);
     return hipGetLastError();
 }
 
@@ -369,9 +378,7 @@ extern "C" int hstu_hip_gated_linear(const hstu_gated_params* p, void* workspace
     if (rc != HSTU_OK) return rc;
     char* ws = reinterpret_cast<char*>(workspace);
     const int64_t ld = padded(p->k, p->dtype);
-    hipError_t e = hipSuccess;
-    if (l.pad_x) e = launch_pad(p->dtype, p->x, p->x_stride, p->m, p->k, ws + l.x, ld, st);
-    if (e == hipSuccess && l.pad_w) e = launch_pad(p->dtype, p->weight, p->k, 2 * (int64_t)p->f, p->k, ws + l.w, ld, st);
+    hipError_t e = launch_pad(p->dtype, p->x, p->x_stride, p->m, l.pad_x ? ws + l.x : nullptr, p->weight, 2 * (int64_t)p->f, l.pad_w ? ws + l.w : nullptr, p->k, ld, st);
     if (e == hipSuccess) {
         GemmArgs a = {};
         fill(a, pl, p->m, p->f, p->k);
@@ -431,8 +438,8 @@ extern "C" int hstu_hip_gated_linear_backward(const hstu_gated_bwd_params* p, vo
             e = launch_colsum(d.partial, (int)l.row_blocks, p->f, db, db + (int64_t)p->f * elem_bytes(p->grad_bias_dtype), p->grad_bias_dtype, st);
         }
     }
-    if (e == hipSuccess && l.pad_w) e = launch_pad(p->dtype, p->weight, p->k, 2 * (int64_t)p->f, p->k, ws + l.w, l.kld, st);
-    if (e == hipSuccess && l.pad_x) e = launch_pad(p->dtype, p->x, p->x_stride, p->m, p->k, ws + l.x, l.kld, st);
+    if (e == hipSuccess)
+        e = launch_pad(p->dtype, p->x, p->x_stride, p->m, l.pad_x ? ws + l.x : nullptr, p->weight, 2 * (int64_t)p->f, l.pad_w ? ws + l.w : nullptr, p->k, l.kld, st);
     if (e == hipSuccess && p->d_x && p->m > 0) {
         GemmArgs a = {};
         fill(a, l.dx, p->m, p->k, 2 * (int64_t)p->f);

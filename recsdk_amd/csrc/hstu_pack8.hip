@@ -56,7 +56,7 @@ __global__ __launch_bounds__(P8_NT) void hstu_pack8_kernel(const hstu_pack8_para
         for (int i = 0; i < P8_ROWS; i++) {
             const int64_t r = r0 + (int64_t)i * rows_wg;
             if (r >= p.rows || n <= 0) continue;
-            unpack8_any(p.codes + r * p.cols + c, n, p.exponents[r * groups + c / HSTU_PACK8_GROUP], largest_finite<T>(), v[i]);
+            code_values(codes8_raw(p.codes + r * p.cols + c, n, p.exponents[r * groups + c / HSTU_PACK8_GROUP]), largest_finite<T>(), v[i]);
         }
 #pragma unroll
         for (int i = 0; i < P8_ROWS; i++) {
