@@ -105,24 +105,53 @@ __global__ __launch_bounds__(256) void hstu_gated_dz_kernel(const DzArgs a) {
     }
 }
 
-// ---- sums over the shares of a contraction -------------------------------------------------------------------------------
+// ---- partial sums ----------------------------------------------------------------------------------------------------------
+// What the launches before it left in fp32 parts: shares of d_x and of d_weight, and the row blocks' column sums for d_bias, added
+// in order and rounded once, all three in one launch.  A lane adds four neighbouring elements over the parts; where there are
+// many (`slots` = 32), lane groups take every 32nd part and meet in LDS.  d_bias, with the most parts, comes first.
+struct SumArgs {
+    const float* part[3];
+    void* out[3];
+    int64_t n[3];        // elements
+    int64_t blocks[3];   // workgroups
+    int32_t parts[3];
+    int32_t slots[3];    // 1 or 32
+    int32_t bias_f32;    // the first output's type
+};
 template <typename T>
-__global__ __launch_bounds__(256) void hstu_sum_splits_kernel(const float* partial, int splits, int64_t n, T* out) {
-    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (int64_t)gridDim.x * 1024) {
-        if (i + 4 <= n) {
-            typedef gm_f32x4 __attribute__((aligned(4))) f4;
-            gm_f32x4 s = *reinterpret_cast<const f4*>(partial + i);
-            for (int k = 1; k < splits; k++) s += *reinterpret_cast<const f4*>(partial + k * n + i);
+__global__ __launch_bounds__(256) void hstu_sum_parts_kernel(const SumArgs a) {
+    __shared__ gm_f32x4 red[256];
+    int64_t block = blockIdx.x;
+    int w = 0;
+    while (w < 2 && block >= a.blocks[w]) block -= a.blocks[w++];
+    const int slots = a.slots[w], across = 256 / slots, slot = threadIdx.x / across;
+    const int64_t n = a.n[w], i = (block * across + threadIdx.x % across) * 4;
+    typedef gm_f32x4 __attribute__((aligned(4))) f4;
+    gm_f32x4 s = {0.f, 0.f, 0.f, 0.f};
+    if (i + 4 <= n) {
+#pragma unroll 8
+        for (int k = slot; k < a.parts[w]; k += slots) s += *reinterpret_cast<const f4*>(a.part[w] + k * n + i);
+    } else {
+        for (int k = slot; k < a.parts[w]; k += slots)
 #pragma unroll
-            for (int k = 0; k < 4; k++) out[i + k] = from_float<T>(s[k]);
-        } else {
-            for (int64_t j = i; j < n; j++) {
-                float s = partial[j];
-                for (int k = 1; k < splits; k++) s += partial[k * n + j];
-                out[j] = from_float<T>(s);
-            }
-        }
+            for (int e = 0; e < 3; e++)
+                if (i + e < n) s[e] += a.part[w][k * n + i + e];
     }
+    if (slots > 1) {
+        red[threadIdx.x] = s;
+        for (int h = slots / 2; h > 0; h >>= 1) {
+            __syncthreads();
+            if (slot < h) red[threadIdx.x] += red[threadIdx.x + h * across];
+        }
+        if (slot) return;
+        s = red[threadIdx.x];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        if (i + e < n) {
+            if (w == 0 && a.bias_f32) reinterpret_cast<float*>(a.out[w])[i + e] = s[e];
+            else reinterpret_cast<T*>(a.out[w])[i + e] = from_float<T>(s[e]);
+        }
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------
@@ -266,7 +295,7 @@ struct GatedBwdLayout {
     Plan dx, dw;
     int64_t ld, kld;                 // rows of dz, padded rows of x / weight
     bool need_dz, pad_x, pad_w;
-    uint64_t dz, x, w, parts, sums, bytes;
+    uint64_t dz, x, w, parts_x, parts_w, sums, bytes;
     int lanes, col_blocks;
     int64_t rows_wg, row_blocks;
 };
@@ -298,11 +327,10 @@ static GatedBwdLayout gated_bwd_layout(const hstu_gated_bwd_params* p) {
     if (l.pad_x) at += up256((uint64_t)p->m * l.kld * e);
     l.w = at;
     if (l.pad_w) at += up256(2 * (uint64_t)p->f * l.kld * e);
-    l.parts = at;
-    uint64_t parts = 0;
-    if (p->d_x && l.dx.splits > 1) parts = (uint64_t)l.dx.splits * p->m * p->k * 4;
-    if (p->d_weight && l.dw.splits > 1) { const uint64_t q = (uint64_t)l.dw.splits * 2 * p->f * p->k * 4; parts = q > parts ? q : parts; }
-    at += up256(parts);
+    l.parts_x = at;
+    if (p->d_x && l.dx.splits > 1) at += up256((uint64_t)l.dx.splits * p->m * p->k * 4);
+    l.parts_w = at;
+    if (p->d_weight && l.dw.splits > 1) at += up256((uint64_t)l.dw.splits * 2 * p->f * p->k * 4);
     l.sums = at;
     if (p->d_bias) at += up256((uint64_t)l.row_blocks * 2 * p->f * 4);
     l.bytes = at;
@@ -336,12 +364,24 @@ static int check_workspace(void* ws, uint64_t have, uint64_t need) {
     return HSTU_OK;
 }
 
-static hipError_t sum_splits(int32_t dtype, const float* partial, int splits, int64_t n, void* out, hipStream_t st) {
-    const int64_t want = (n + 1023) / 1024;
-    const dim3 grid((unsigned)(want > 4096 ? 4096 : want));
-    if (dtype == HSTU_F32) hipLaunchKernelGGL(hstu_sum_splits_kernel<float>, grid, dim3(256), 0, st, partial, splits, n, (float*)out);
-    else if (dtype == HSTU_F16) hipLaunchKernelGGL(hstu_sum_splits_kernel<_Float16>, grid, dim3(256), 0, st, partial, splits, n, (_Float16*)out);
-    else hipLaunchKernelGGL(hstu_sum_splits_kernel<__bf16>, grid, dim3(256), 0, st, partial, splits, n, (__bf16*)out);
+static void add_sum(SumArgs& a, int which, const void* part, int64_t parts, int64_t n, void* out) {
+    a.part[which] = reinterpret_cast<const float*>(part);
+    a.parts[which] = (int32_t)parts;
+    a.n[which] = n;
+    a.out[which] = out;
+    a.slots[which] = parts > 16 ? 32 : 1;
+    const int64_t per = 256 / a.slots[which] * 4;
+    a.blocks[which] = (n + per - 1) / per;
+}
+static hipError_t launch_sums(int32_t dtype, SumArgs& a, hipStream_t st) {
+    const int64_t blocks = a.blocks[0] + a.blocks[1] + a.blocks[2];
+    if (blocks == 0) return hipSuccess;
+    for (int i = 0; i < 3; i++)
+        if (!a.slots[i]) a.slots[i] = 1;
+    const dim3 grid((unsigned)blocks);
+    if (dtype == HSTU_F32) hipLaunchKernelGGL(hstu_sum_parts_kernel<float>, grid, dim3(256), 0, st, a);
+    else if (dtype == HSTU_F16) hipLaunchKernelGGL(hstu_sum_parts_kernel<_Float16>, grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(hstu_sum_parts_kernel<__bf16>, grid, dim3(256), 0, st, a);
     return hipGetLastError();
 }
 
@@ -418,6 +458,8 @@ extern "C" int hstu_hip_gated_linear_backward(const hstu_gated_bwd_params* p, vo
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     char* ws = reinterpret_cast<char*>(workspace);
     hipError_t e = hipSuccess;
+    SumArgs sums = {};
+    sums.bias_f32 = p->grad_bias_dtype == HSTU_F32;
     if (l.need_dz || p->d_bias) {
         DzArgs d = {};
         d.d_out = p->d_out; d.z = p->z; d.z_exp = p->z_exponents;
@@ -433,7 +475,10 @@ extern "C" int hstu_hip_gated_linear_backward(const hstu_gated_bwd_params* p, vo
         else if (p->dtype == HSTU_F16) hipLaunchKernelGGL(hstu_gated_dz_kernel<_Float16>, grid, dim3(256), 0, st, d);
         else hipLaunchKernelGGL(hstu_gated_dz_kernel<__bf16>, grid, dim3(256), 0, st, d);
         e = hipGetLastError();
-        if (e == hipSuccess && p->d_bias) {
+        // where a product leaves parts too, the column sums are added in the same launch as those; alone, while they are in the L2
+        const bool parts = (p->d_x && p->m > 0 && l.dx.splits > 1) || (p->d_weight && l.dw.splits > 1);
+        if (p->d_bias && parts) add_sum(sums, 0, d.partial, l.row_blocks, 2 * (int64_t)p->f, p->d_bias);
+        else if (e == hipSuccess && p->d_bias) {
             char* db = reinterpret_cast<char*>(p->d_bias);
             e = launch_colsum(d.partial, (int)l.row_blocks, p->f, db, db + (int64_t)p->f * elem_bytes(p->grad_bias_dtype), p->grad_bias_dtype, st);
         }
@@ -447,9 +492,9 @@ extern "C" int hstu_hip_gated_linear_backward(const hstu_gated_bwd_params* p, vo
         a.n_ld = l.pad_w ? l.kld : p->k;
         a.m_op = ws + l.dz;
         a.m_ld = l.ld;
-        a.out = l.dx.splits > 1 ? ws + l.parts : p->d_x;
+        a.out = l.dx.splits > 1 ? ws + l.parts_x : p->d_x;
         e = launch_gemm(p->dtype, a, GEMM_DX, l.dx.tile, st);
-        if (e == hipSuccess && l.dx.splits > 1) e = sum_splits(p->dtype, reinterpret_cast<float*>(ws + l.parts), l.dx.splits, p->m * p->k, p->d_x, st);
+        if (l.dx.splits > 1) add_sum(sums, 1, ws + l.parts_x, l.dx.splits, p->m * p->k, p->d_x);
     }
     if (e == hipSuccess && p->d_weight) {
         // without rows the product of empty sums writes zeros
@@ -459,10 +504,11 @@ extern "C" int hstu_hip_gated_linear_backward(const hstu_gated_bwd_params* p, vo
         a.n_ld = l.pad_x ? l.kld : p->m > 1 ? p->x_stride : l.kld;
         a.m_op = ws + l.dz;
         a.m_ld = l.ld;
-        a.out = l.dw.splits > 1 ? ws + l.parts : p->d_weight;
+        a.out = l.dw.splits > 1 ? ws + l.parts_w : p->d_weight;
         e = launch_gemm(p->dtype, a, GEMM_DW, l.dw.tile, st);
-        if (e == hipSuccess && l.dw.splits > 1) e = sum_splits(p->dtype, reinterpret_cast<float*>(ws + l.parts), l.dw.splits, 2 * (int64_t)p->f * p->k, p->d_weight, st);
+        if (l.dw.splits > 1) add_sum(sums, 2, ws + l.parts_w, l.dw.splits, 2 * (int64_t)p->f * p->k, p->d_weight);
     }
+    if (e == hipSuccess) e = launch_sums(p->dtype, sums, st);
     if (e != hipSuccess) return fail(HSTU_ERR_LAUNCH, "kernel launch failed: %s", hipGetErrorString(e));
     return HSTU_OK;
 }
