@@ -92,15 +92,17 @@ int hstu_hip_activation_unpack8(const hstu_pack8_params* p, void* stream);
 /* Gated projection:
  *   z = x W^T + bias     [m, 2 f], fp32 accumulation; weight rows and z columns [0, f) are the gate, [f, 2 f) the values
  *   out = round(act(z[:, :f]) * z[:, f:])
- * keep says what the backward gets: nothing, z rounded to dtype, or z in 8 bits (the groups of the two halves do not mix:
- * exponents are [m, 2, ceil(f / 32)]).  m may be 0. */
+ * keep says what the backward gets: nothing, z, or z in 8 bits.  z is kept in fp32 for HSTU_F32 and in 24 bits otherwise: the upper
+ * 16 bits of the fp32 value in z, the next 8 in z_aux (1 + 8 + 15 bits; rounded to 16 bits, z alone would put as large an error into
+ * the gradients as the rounding of dz and of the gradients themselves).  In 8 bits the groups of the two halves do not mix: the
+ * exponents in z_aux are [m, 2, ceil(f / 32)].  m may be 0. */
 #define HSTU_GATED_MAX_K 16384
 #define HSTU_GATED_MAX_F 32768
 enum { HSTU_ACT_SILU = 0, HSTU_ACT_GELU = 1 /* z * Phi(z), with erf */ };
 enum { HSTU_KEEP_NONE = 0, HSTU_KEEP_FULL = 1, HSTU_KEEP_8BIT = 2 /* 16-bit dtypes only */ };
 typedef struct hstu_gated_params {
     uint32_t struct_size;
-    int32_t dtype;         /* HSTU_F32 / HSTU_F16 / HSTU_BF16: x, weight, out, z */
+    int32_t dtype;         /* HSTU_F32 / HSTU_F16 / HSTU_BF16: x, weight, out */
     int32_t bias_dtype;    /* dtype or HSTU_F32 */
     int32_t act;
     int32_t keep;
@@ -113,8 +115,8 @@ typedef struct hstu_gated_params {
     const void* weight;    /* [2 f, k], contiguous */
     const void* bias;      /* [2 f], or NULL */
     void* out;             /* [m, f], contiguous */
-    void* z;               /* HSTU_KEEP_FULL: [m, 2 f]; HSTU_KEEP_8BIT: codes [m, 2 f] */
-    uint8_t* z_exponents;  /* HSTU_KEEP_8BIT */
+    void* z;               /* HSTU_KEEP_FULL: [m, 2 f] fp32 or 16-bit upper parts; HSTU_KEEP_8BIT: codes [m, 2 f] */
+    uint8_t* z_aux;        /* HSTU_KEEP_FULL of 16-bit dtypes: lower parts [m, 2 f]; HSTU_KEEP_8BIT: exponents */
 } hstu_gated_params;
 int hstu_hip_gated_linear_get_workspace_size(const hstu_gated_params* p, uint64_t* workspace_bytes);
 int hstu_hip_gated_linear(const hstu_gated_params* p, void* workspace, uint64_t workspace_bytes, void* stream);
@@ -138,7 +140,7 @@ typedef struct hstu_gated_bwd_params {
     const void* x;            /* [m, k]; read for d_weight only */
     const void* weight;       /* [2 f, k]; read for d_x only */
     const void* z;
-    const uint8_t* z_exponents;
+    const uint8_t* z_aux;
     void* d_x;                /* [m, k], contiguous */
     void* d_weight;           /* [2 f, k], contiguous */
     void* d_bias;             /* [2 f] */

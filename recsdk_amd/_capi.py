@@ -175,7 +175,7 @@ class HstuGatedParams(C.Structure):
         ("struct_size", C.c_uint32), ("dtype", C.c_int32), ("bias_dtype", C.c_int32), ("act", C.c_int32), ("keep", C.c_int32),
         ("k", C.c_int32), ("f", C.c_int32), ("reserved", C.c_uint32), ("m", C.c_int64), ("x_stride", C.c_int64),
         ("x", C.c_void_p), ("weight", C.c_void_p), ("bias", C.c_void_p), ("out", C.c_void_p), ("z", C.c_void_p),
-        ("z_exponents", C.c_void_p),
+        ("z_aux", C.c_void_p),
     ]
 
 
@@ -184,7 +184,7 @@ class HstuGatedBwdParams(C.Structure):
         ("struct_size", C.c_uint32), ("dtype", C.c_int32), ("grad_bias_dtype", C.c_int32), ("act", C.c_int32), ("keep", C.c_int32),
         ("k", C.c_int32), ("f", C.c_int32), ("reserved", C.c_uint32), ("m", C.c_int64), ("x_stride", C.c_int64),
         ("dout_stride", C.c_int64), ("d_out", C.c_void_p), ("x", C.c_void_p), ("weight", C.c_void_p), ("z", C.c_void_p),
-        ("z_exponents", C.c_void_p), ("d_x", C.c_void_p), ("d_weight", C.c_void_p), ("d_bias", C.c_void_p),
+        ("z_aux", C.c_void_p), ("d_x", C.c_void_p), ("d_weight", C.c_void_p), ("d_bias", C.c_void_p),
     ]
 
 

@@ -120,6 +120,23 @@ __device__ __forceinline__ void act_and_grad(float z, int act, float& a, float& 
     }
 }
 
+// ---- z in 24 bits: the upper 16 bits of an fp32 value in one plane, the next 8 in another -------------------------------------
+// (the rest is cut off: 2^-15 of the value at most, and a NaN of the arithmetic stays one)
+__device__ __forceinline__ unsigned upper_pair(float a, float b) { return __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, b), __builtin_bit_cast(unsigned, a), 0x07060302u); }
+__device__ __forceinline__ unsigned lower_quad(float a, float b, float c, float d) {
+    const unsigned lo = __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, b), __builtin_bit_cast(unsigned, a), 0x0c0c0501u);
+    const unsigned hi = __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, d), __builtin_bit_cast(unsigned, c), 0x05010c0cu);
+    return lo | hi;
+}
+// 8 values from 8 upper parts and 8 lower ones
+__device__ __forceinline__ void join24(const ffn_u4& up, const ffn_u2& low, float* v) {
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+        const unsigned u = k & 1 ? up[k >> 1] & 0xffff0000u : up[k >> 1] << 16, l = (low[k >> 2] >> (8 * (k & 3))) & 0xffu;
+        v[k] = __builtin_bit_cast(float, u | (l << 8));
+    }
+}
+
 // ---- 8-bit activations ---------------------------------------------------------------------------------------------------
 // exponent byte of a group whose finite values reach `top` (>= 0): 448 = 1.75 * 2^8, so E = floor(log2 top) - 8, one more
 // where the mantissa is above 1.75

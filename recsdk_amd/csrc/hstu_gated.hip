@@ -2,7 +2,7 @@
 // tiles, and the row work around the matrix products of hstu_gemm.h.
 //   forward   one product kernel whose waves hold a block of the gate and the matching block of the values, so that
 //             activation and product happen on the accumulators
-//   backward  dz from d_out and the kept z (one pass, also the column sums for d_bias), then d_x = dz W and d_weight = dz^T x,
+//   backward  dz from d_out and the kept z (24 bits; one pass, also the column sums for d_bias), then d_x = dz W and d_weight = dz^T x,
 //             which read their operands as they lie in memory (transposing LDS reads; nothing is transposed in HBM)
 // dz is rounded to the I/O type between the two: the products run on the 16-bit matrix cores, and the rounding (2^-9 relative
 // per element, independent) averages out over sums of 2 f and of m terms.
@@ -35,7 +35,7 @@ __global__ __launch_bounds__(256) void hstu_pad_rows_kernel(const PadArgs a) {
 struct DzArgs {
     const void* d_out;
     const void* z;
-    const uint8_t* z_exp;
+    const uint8_t* z_aux;
     void* dz;              // [m, ld], or NULL
     float* partial;        // [row blocks, 2 f] column sums, or NULL
     int64_t m, dout_stride, ld;
@@ -61,13 +61,20 @@ __global__ __launch_bounds__(256) void hstu_gated_dz_kernel(const DzArgs a) {
             load8_any(reinterpret_cast<const T*>(a.d_out) + r * a.dout_stride + c, n, d);
             if (a.keep == HSTU_KEEP_8BIT) {
                 const uint8_t* z = reinterpret_cast<const uint8_t*>(a.z) + r * 2 * a.f + c;
-                const uint8_t* e = a.z_exp + r * 2 * groups + c / HSTU_PACK8_GROUP;
+                const uint8_t* e = a.z_aux + r * 2 * groups + c / HSTU_PACK8_GROUP;
                 code_values(codes8_raw(z, n, e[0]), largest_finite<float>(), zg);
                 code_values(codes8_raw(z + a.f, n, e[groups]), largest_finite<float>(), zu);
-            } else {
+            } else if constexpr (sizeof(T) == 4) {
                 const T* z = reinterpret_cast<const T*>(a.z) + r * 2 * a.f + c;
                 load8_any(z, n, zg);
                 load8_any(z + a.f, n, zu);
+            } else {
+                const T* z = reinterpret_cast<const T*>(a.z) + r * 2 * a.f + c;
+                const uint8_t* low = a.z_aux + r * 2 * a.f + c;
+                const Raw8<T> ug = load8_raw(z, n), uu = load8_raw(z + a.f, n);
+                const Codes8 lg = codes8_raw(low, n, 0), lu = codes8_raw(low + a.f, n, 0);
+                join24(ug.q[0], lg.q, zg);
+                join24(uu.q[0], lu.q, zu);
             }
             float dg[8], du[8];
 #pragma unroll
@@ -283,8 +290,8 @@ static int gated_validate(const hstu_gated_params* p) {
     if (p->x_stride < 0) return fail(HSTU_ERR_INVALID_ARGUMENT, "x_stride must not be negative");
     if (p->m == 0) return HSTU_OK;
     if (!p->x || !p->weight || !p->out) return fail(HSTU_ERR_INVALID_ARGUMENT, "x, weight and out must not be NULL");
-    if ((p->keep != HSTU_KEEP_NONE && !p->z) || (p->keep == HSTU_KEEP_8BIT && !p->z_exponents))
-        return fail(HSTU_ERR_INVALID_ARGUMENT, "z (and z_exponents for 8 bits) must not be NULL when they are kept");
+    if (p->keep != HSTU_KEEP_NONE && (!p->z || (p->dtype != HSTU_F32 && !p->z_aux)))
+        return fail(HSTU_ERR_INVALID_ARGUMENT, "z (and z_aux for 16-bit dtypes) must not be NULL when z is kept");
     if (bad_align(p->x, p->dtype) || bad_align(p->weight, p->dtype) || bad_align(p->out, p->dtype) || bad_align(p->bias, p->bias_dtype) ||
         (p->keep == HSTU_KEEP_FULL && bad_align(p->z, p->dtype)))
         return fail(HSTU_ERR_UNSUPPORTED, "x, weight, bias, out and z must be aligned to their element types");
@@ -348,8 +355,8 @@ static int gated_bwd_validate(const hstu_gated_bwd_params* p) {
         return fail(HSTU_ERR_INVALID_ARGUMENT, "grad_bias_dtype expect float32 or the dtype of x, but value is %d", p->grad_bias_dtype);
     if (p->x_stride < 0 || p->dout_stride < 0) return fail(HSTU_ERR_INVALID_ARGUMENT, "x_stride and dout_stride must not be negative");
     if (p->m > 0) {
-        if (!p->d_out || !p->z || (p->keep == HSTU_KEEP_8BIT && !p->z_exponents))
-            return fail(HSTU_ERR_INVALID_ARGUMENT, "d_out and z (and z_exponents for 8 bits) must not be NULL");
+        if (!p->d_out || !p->z || (p->dtype != HSTU_F32 && !p->z_aux))
+            return fail(HSTU_ERR_INVALID_ARGUMENT, "d_out and z (and z_aux for 16-bit dtypes) must not be NULL");
         if ((p->d_weight && !p->x) || (p->d_x && !p->weight)) return fail(HSTU_ERR_INVALID_ARGUMENT, "x (for d_weight) and weight (for d_x) must not be NULL");
     }
     if (bad_align(p->d_out, p->dtype) || bad_align(p->x, p->dtype) || bad_align(p->weight, p->dtype) || bad_align(p->d_x, p->dtype) ||
@@ -406,7 +413,7 @@ extern "C" int hstu_hip_gated_linear(const hstu_gated_params* p, void* workspace
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     if (few_rows(p)) {
         RowsArgs a = {};
-        a.x = p->x; a.weight = p->weight; a.bias = p->bias; a.out = p->out; a.z = p->z; a.z_exp = p->z_exponents;
+        a.x = p->x; a.weight = p->weight; a.bias = p->bias; a.out = p->out; a.z = p->z; a.z_aux = p->z_aux;
         a.x_stride = p->x_stride;
         a.m = (int32_t)p->m; a.k = p->k; a.f = p->f; a.bias_f32 = p->bias_dtype == HSTU_F32; a.act = p->act; a.keep = p->keep;
         const hipError_t e = p->dtype == HSTU_F32 ? launch_gated_rows_f32(a, st) : p->dtype == HSTU_F16 ? launch_gated_rows_f16(a, st) : launch_gated_rows_bf16(a, st);
@@ -432,7 +439,7 @@ extern "C" int hstu_hip_gated_linear(const hstu_gated_params* p, void* workspace
         a.act = p->act;
         a.keep = p->keep;
         a.z = p->z;
-        a.z_exp = p->z_exponents;
+        a.z_aux = p->z_aux;
         e = launch_gemm(p->dtype, a, GEMM_GATED, pl.tile, st);
     }
     if (e != hipSuccess) return fail(HSTU_ERR_LAUNCH, "kernel launch failed: %s", hipGetErrorString(e));
@@ -462,7 +469,7 @@ extern "C" int hstu_hip_gated_linear_backward(const hstu_gated_bwd_params* p, vo
     sums.bias_f32 = p->grad_bias_dtype == HSTU_F32;
     if (l.need_dz || p->d_bias) {
         DzArgs d = {};
-        d.d_out = p->d_out; d.z = p->z; d.z_exp = p->z_exponents;
+        d.d_out = p->d_out; d.z = p->z; d.z_aux = p->z_aux;
         d.dz = l.need_dz ? ws + l.dz : nullptr;
         d.partial = p->d_bias ? reinterpret_cast<float*>(ws + l.sums) : nullptr;
         d.m = p->m; d.dout_stride = p->dout_stride; d.ld = l.ld; d.rows_wg = l.rows_wg;

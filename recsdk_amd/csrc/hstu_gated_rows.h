@@ -16,7 +16,7 @@ struct RowsArgs {
     const void* bias;
     void* out;
     void* z;
-    uint8_t* z_exp;
+    uint8_t* z_aux;
     int64_t x_stride;
     int32_t m, k, f, bias_f32, act, keep;
 };
@@ -124,9 +124,17 @@ __global__ __launch_bounds__(64 * ROWS_WAVES) void hstu_gated_rows_kernel(const 
         const float zg = zs[0][m][c], zu = zs[1][m][c];
         reinterpret_cast<T*>(a.out)[(int64_t)m * a.f + f] = from_float<T>(act_of(zg, a.act) * zu);
         if (a.keep == HSTU_KEEP_FULL) {
-            T* z = reinterpret_cast<T*>(a.z) + (int64_t)m * 2 * a.f + f;
-            z[0] = from_float<T>(zg);
-            z[a.f] = from_float<T>(zu);
+            const int64_t at = (int64_t)m * 2 * a.f + f;
+            if constexpr (sizeof(T) == 4) {
+                reinterpret_cast<T*>(a.z)[at] = zg;
+                reinterpret_cast<T*>(a.z)[at + a.f] = zu;
+            } else {
+                const unsigned bg = __builtin_bit_cast(unsigned, zg), bu = __builtin_bit_cast(unsigned, zu);
+                reinterpret_cast<uint16_t*>(a.z)[at] = (uint16_t)(bg >> 16);
+                reinterpret_cast<uint16_t*>(a.z)[at + a.f] = (uint16_t)(bu >> 16);
+                a.z_aux[at] = (uint8_t)(bg >> 8);
+                a.z_aux[at + a.f] = (uint8_t)(bu >> 8);
+            }
         }
     }
     if constexpr (FB == 2) {
@@ -137,7 +145,7 @@ __global__ __launch_bounds__(64 * ROWS_WAVES) void hstu_gated_rows_kernel(const 
             const int e = pack8_exponent(top);
             const float inv = pack8_inv_scale(e);
             const int groups = (a.f + HSTU_PACK8_GROUP - 1) / HSTU_PACK8_GROUP;
-            a.z_exp[((int64_t)m * 2 + h) * groups + blockIdx.x] = (uint8_t)e;
+            a.z_aux[((int64_t)m * 2 + h) * groups + blockIdx.x] = (uint8_t)e;
             uint8_t* z = reinterpret_cast<uint8_t*>(a.z) + ((int64_t)m * 2 + h) * a.f + f0;
             for (int c = 0; c < 32; c += 4) {
                 const unsigned u = pack8_codes(zs[h][m][c], zs[h][m][c + 1], zs[h][m][c + 2], zs[h][m][c + 3], inv);

@@ -48,7 +48,7 @@ struct GemmArgs {
     int32_t act;
     int32_t keep;
     void* z;
-    uint8_t* z_exp;
+    uint8_t* z_aux;
 };
 
 template <typename T> struct GM;
@@ -182,17 +182,31 @@ __device__ __forceinline__ typename GM<typename S::T>::frag read_frag(const char
 }
 
 // 16 consecutive n-side values of a lane's row m (register r holds n = 8 (r / 4) + 4 g + r % 4) to memory; `n_left` valid columns
+// as pairs of 16 bits
+template <typename T> __device__ __forceinline__ void store_pairs(T* row, const unsigned* w, int g, int n_left) {
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        unsigned a0 = w[4 * h], a1 = w[4 * h + 1], b0 = w[4 * h + 2], b1 = w[4 * h + 3];
+        swap_halves(a0, b0);
+        swap_halves(a1, b1);
+        const int n = 16 * h + 8 * g;
+        if (n < n_left) store16<T>(row + n, (gm_u4){a0, a1, b0, b1}, n_left - n);
+    }
+}
+// as quads of bytes
+__device__ __forceinline__ void store_quads(uint8_t* row, const unsigned* w, int g, int n_left) {
+    unsigned c0 = w[0], c1 = w[1], c2 = w[2], c3 = w[3];
+    swap_halves(c0, c2);
+    swap_halves(c1, c3);
+    const int n = 16 * g;
+    if (n < n_left) store16<uint8_t>(row + n, (gm_u4){c0, c2, c1, c3}, n_left - n);
+}
 template <typename T> __device__ __forceinline__ void store_block(T* row, const float* v, int g, int n_left) {
     if constexpr (sizeof(T) == 2) {
+        unsigned w[8];
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            unsigned a0 = GM<T>::pack2(v[8 * h], v[8 * h + 1]), a1 = GM<T>::pack2(v[8 * h + 2], v[8 * h + 3]);
-            unsigned b0 = GM<T>::pack2(v[8 * h + 4], v[8 * h + 5]), b1 = GM<T>::pack2(v[8 * h + 6], v[8 * h + 7]);
-            swap_halves(a0, b0);
-            swap_halves(a1, b1);
-            const int n = 16 * h + 8 * g;
-            if (n < n_left) store16<T>(row + n, (gm_u4){a0, a1, b0, b1}, n_left - n);
-        }
+        for (int i = 0; i < 8; i++) w[i] = GM<T>::pack2(v[2 * i], v[2 * i + 1]);
+        store_pairs(row, w, g, n_left);
     } else {
 #pragma unroll
         for (int rr = 0; rr < 4; rr++) {
@@ -363,9 +377,21 @@ __global__ __launch_bounds__(S::NT) void hstu_gemm_kernel(const GemmArgs a) {
             }
             store_block<T>(reinterpret_cast<T*>(a.out) + m * a.N + n, h, g, left);
             if (a.keep == HSTU_KEEP_FULL) {
-                T* z = reinterpret_cast<T*>(a.z) + m * 2 * a.N + n;
-                store_block<T>(z, zg, g, left);
-                store_block<T>(z + a.N, zu, g, left);
+#pragma unroll
+                for (int part = 0; part < 2; part++) {
+                    const float* v = part ? zu : zg;
+                    const int64_t at = (m * 2 + part) * a.N + n;
+                    if constexpr (S::ES == 4) store_block<T>(reinterpret_cast<T*>(a.z) + at, v, g, left);
+                    else {
+                        unsigned up[8], low[4];
+#pragma unroll
+                        for (int i = 0; i < 8; i++) up[i] = upper_pair(v[2 * i], v[2 * i + 1]);
+#pragma unroll
+                        for (int i = 0; i < 4; i++) low[i] = lower_quad(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                        store_pairs(reinterpret_cast<T*>(a.z) + at, up, g, left);
+                        store_quads(a.z_aux + at, low, g, left);
+                    }
+                }
             } else if (a.keep == HSTU_KEEP_8BIT) {
                 // the 32 columns of a row lie in the 16 registers of two lanes; columns past f hold zero (no bias, no weight row)
 #pragma unroll
@@ -380,16 +406,10 @@ __global__ __launch_bounds__(S::NT) void hstu_gemm_kernel(const GemmArgs a) {
                     unsigned c[4];
 #pragma unroll
                     for (int rr = 0; rr < 4; rr++) c[rr] = pack8_codes(v[4 * rr], v[4 * rr + 1], v[4 * rr + 2], v[4 * rr + 3], inv);
-                    swap_halves(c[0], c[2]);
-                    swap_halves(c[1], c[3]);
-                    const int nn = 16 * g;
-                    if (nn < left) {
-                        uint8_t* z = reinterpret_cast<uint8_t*>(a.z) + m * 2 * a.N + (part ? a.N : 0) + n + nn;
-                        store16<uint8_t>(z, (gm_u4){c[0], c[2], c[1], c[3]}, left - nn);
-                    }
+                    store_quads(reinterpret_cast<uint8_t*>(a.z) + (m * 2 + part) * a.N + n, c, g, left);
                     if (g == 0 && left > 0) {
                         const int groups = (a.N + HSTU_PACK8_GROUP - 1) / HSTU_PACK8_GROUP;
-                        a.z_exp[(m * 2 + part) * groups + n / HSTU_PACK8_GROUP] = (uint8_t)e;
+                        a.z_aux[(m * 2 + part) * groups + n / HSTU_PACK8_GROUP] = (uint8_t)e;
                     }
                 }
             }

@@ -250,7 +250,12 @@ static std::vector<int64_t> with_last(const at::Tensor& x, int64_t last) {
     return s;
 }
 
-// {out}, {out, z} or {out, codes, exponents}
+// what the first plane of a kept z is typed as
+static at::ScalarType kept_type(const at::Tensor& x, bool checkpoint8) {
+    return checkpoint8 ? at::kFloat8_e4m3fn : x.scalar_type() == at::kFloat ? at::kFloat : at::kBFloat16;
+}
+
+// {out}, {out, z} (fp32), {out, upper parts of z, lower parts} (16-bit types: z in 24 bits) or {out, codes, exponents}
 static std::vector<at::Tensor> gl_forward(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& bias, int32_t act, int32_t keep) {
     gl_check(x, weight, bias, keep == HSTU_KEEP_8BIT);
     check_devices(GL, {&x, &weight, &bias});
@@ -258,8 +263,9 @@ static std::vector<at::Tensor> gl_forward(const at::Tensor& x, const at::Tensor&
     const at::Tensor xr = rows_of(x), w = weight.contiguous(), b = bias.defined() ? bias.contiguous() : bias;
     const int64_t m = row_count(x), f = weight.size(0) / 2, groups = (f + HSTU_PACK8_GROUP - 1) / HSTU_PACK8_GROUP;
     std::vector<at::Tensor> outs{at::empty(with_last(x, f), x.options().memory_format(at::MemoryFormat::Contiguous))};
-    if (keep != HSTU_KEEP_NONE) outs.push_back(at::empty({m, 2 * f}, x.options().dtype(keep == HSTU_KEEP_8BIT ? at::kFloat8_e4m3fn : x.scalar_type())));
+    if (keep != HSTU_KEEP_NONE) outs.push_back(at::empty({m, 2 * f}, x.options().dtype(kept_type(x, keep == HSTU_KEEP_8BIT))));
     if (keep == HSTU_KEEP_8BIT) outs.push_back(at::empty({m, 2, groups}, x.options().dtype(at::kByte)));
+    else if (keep == HSTU_KEEP_FULL && x.scalar_type() != at::kFloat) outs.push_back(at::empty({m, 2 * f}, x.options().dtype(at::kByte)));
     hstu_gated_params p;
     std::memset(&p, 0, sizeof(p));
     p.struct_size = sizeof(p);
@@ -276,7 +282,7 @@ static std::vector<at::Tensor> gl_forward(const at::Tensor& x, const at::Tensor&
     p.bias = b.defined() ? b.const_data_ptr() : nullptr;
     p.out = outs[0].data_ptr();
     p.z = keep != HSTU_KEEP_NONE ? outs[1].data_ptr() : nullptr;
-    p.z_exponents = keep == HSTU_KEEP_8BIT ? outs[2].data_ptr<uint8_t>() : nullptr;
+    p.z_aux = outs.size() > 2 ? outs[2].data_ptr<uint8_t>() : nullptr;
     uint64_t bytes = 0;
     int rc = hstu_hip_gated_linear_get_workspace_size(&p, &bytes);
     TORCH_CHECK(rc == HSTU_OK, GL, ": ", hstu_hip_last_error());
@@ -288,11 +294,11 @@ static std::vector<at::Tensor> gl_forward(const at::Tensor& x, const at::Tensor&
 }
 
 // {d_x, d_weight, d_bias}, undefined where not wanted
-static std::vector<at::Tensor> gl_backward(const at::Tensor& d_out, const at::Tensor& x, const at::Tensor& weight, const at::Tensor& z, const at::Tensor& exps,
+static std::vector<at::Tensor> gl_backward(const at::Tensor& d_out, const at::Tensor& x, const at::Tensor& weight, const at::Tensor& z, const at::Tensor& aux,
                                            int32_t act, at::ScalarType bias_type, bool want_x, bool want_w, bool want_b) {
-    check_devices(GL, {&x, &weight, &d_out, &z, &exps});
+    check_devices(GL, {&x, &weight, &d_out, &z, &aux});
     Launch launch(x);
-    const at::Tensor xr = rows_of(x), gr = rows_of(d_out), w = weight.contiguous(), zc = z.contiguous(), ec = exps.defined() ? exps.contiguous() : exps;
+    const at::Tensor xr = rows_of(x), gr = rows_of(d_out), w = weight.contiguous(), zc = z.contiguous(), ac = aux.defined() ? aux.contiguous() : aux;
     const int64_t m = row_count(x), f = weight.size(0) / 2;
     at::Tensor dx, dw, db;
     if (want_x) dx = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
@@ -304,7 +310,7 @@ static std::vector<at::Tensor> gl_backward(const at::Tensor& d_out, const at::Te
     p.dtype = type_code(x.scalar_type(), GL, "x");
     p.grad_bias_dtype = type_code(bias_type, GL, "bias");
     p.act = act;
-    p.keep = exps.defined() ? HSTU_KEEP_8BIT : HSTU_KEEP_FULL;
+    p.keep = z.scalar_type() == at::kFloat8_e4m3fn ? HSTU_KEEP_8BIT : HSTU_KEEP_FULL;
     p.k = (int32_t)x.size(-1);
     p.f = (int32_t)f;
     p.m = m;
@@ -314,7 +320,7 @@ static std::vector<at::Tensor> gl_backward(const at::Tensor& d_out, const at::Te
     p.x = xr.const_data_ptr();
     p.weight = w.const_data_ptr();
     p.z = zc.const_data_ptr();
-    p.z_exponents = ec.defined() ? (const uint8_t*)ec.const_data_ptr() : nullptr;
+    p.z_aux = ac.defined() ? (const uint8_t*)ac.const_data_ptr() : nullptr;
     p.d_x = want_x ? dx.data_ptr() : nullptr;
     p.d_weight = want_w ? dw.data_ptr() : nullptr;
     p.d_bias = want_b ? db.data_ptr() : nullptr;
@@ -335,7 +341,7 @@ public:
         at::AutoDispatchBelowADInplaceOrView guard;
         const at::Tensor bias = value(bias_);
         auto outs = gl_forward(x, weight, bias, (int32_t)act, checkpoint8 ? HSTU_KEEP_8BIT : HSTU_KEEP_FULL);
-        ctx->save_for_backward({x, weight, outs[1], checkpoint8 ? outs[2] : at::Tensor()});
+        ctx->save_for_backward({x, weight, outs[1], outs.size() > 2 ? outs[2] : at::Tensor()});
         ctx->saved_data["act"] = act;
         ctx->saved_data["has_bias"] = bias.defined();
         ctx->saved_data["bias_type"] = (int64_t)(bias.defined() ? bias.scalar_type() : x.scalar_type());
@@ -368,15 +374,18 @@ std::vector<at::Tensor> gated_linear_forward(const at::Tensor& x, const at::Tens
     return gl_forward(x, weight, value(bias), act_code(activation), checkpoint8 ? HSTU_KEEP_8BIT : HSTU_KEEP_FULL);
 }
 std::vector<at::Tensor> gated_linear_backward(const at::Tensor& d_out, const at::Tensor& x, const at::Tensor& weight, const at::Tensor& z,
-                                              const c10::optional<at::Tensor>& z_exponents, c10::string_view activation) {
-    const at::Tensor e = value(z_exponents);
-    gl_check(x, weight, at::Tensor(), e.defined());
+                                              const c10::optional<at::Tensor>& z_aux, c10::string_view activation) {
+    const at::Tensor aux = value(z_aux);
+    const bool c8 = z.scalar_type() == at::kFloat8_e4m3fn;
+    gl_check(x, weight, at::Tensor(), c8);
     const int64_t m = row_count(x), f = weight.size(0) / 2, groups = (f + HSTU_PACK8_GROUP - 1) / HSTU_PACK8_GROUP;
     TORCH_CHECK(d_out.scalar_type() == x.scalar_type() && d_out.sizes().vec() == with_last(x, f), GL, ": d_out must have the dtype of x and the shape of out");
-    TORCH_CHECK(z.numel() == m * 2 * f && z.scalar_type() == (e.defined() ? at::kFloat8_e4m3fn : x.scalar_type()), GL,
-                ": z must hold [rows, 2 f] values in the dtype of x, or in float8_e4m3fn with z_exponents");
-    if (e.defined()) TORCH_CHECK(e.scalar_type() == at::kByte && e.numel() == m * 2 * groups, GL, ": z_exponents must be uint8 [rows, 2, ceil(f / 32)]");
-    return gl_backward(d_out, x, weight, z, e, act_code(activation), at::kFloat, true, true, true);
+    TORCH_CHECK(z.numel() == m * 2 * f && z.scalar_type() == kept_type(x, c8), GL, ": z must be what gated_linear_forward kept: ", m, " x ", 2 * f,
+                " values, float32 for float32 rows, bfloat16 upper parts or float8_e4m3fn codes otherwise");
+    const int64_t want = c8 ? m * 2 * groups : x.scalar_type() == at::kFloat ? 0 : m * 2 * f;
+    TORCH_CHECK(want == 0 || (aux.defined() && aux.scalar_type() == at::kByte && aux.numel() == want), GL,
+                ": z_aux must be what gated_linear_forward kept beside z: uint8, ", want, " values");
+    return gl_backward(d_out, x, weight, z, want ? aux : at::Tensor(), act_code(activation), at::kFloat, true, true, true);
 }
 
 // ---- 8-bit activations ---------------------------------------------------------------------------------------------------
@@ -437,7 +446,7 @@ TORCH_LIBRARY_FRAGMENT(mxrec, m) {
     m.def("layer_norm_backward(Tensor d_out, Tensor x, Tensor? weight, Tensor mean, Tensor rstd) -> Tensor[]");
     m.def("gated_linear(Tensor x, Tensor weight, Tensor? bias=None, str activation='silu', bool checkpoint8=False) -> Tensor");
     m.def("gated_linear_forward(Tensor x, Tensor weight, Tensor? bias=None, str activation='silu', bool checkpoint8=False) -> Tensor[]");
-    m.def("gated_linear_backward(Tensor d_out, Tensor x, Tensor weight, Tensor z, Tensor? z_exponents=None, str activation='silu') -> Tensor[]");
+    m.def("gated_linear_backward(Tensor d_out, Tensor x, Tensor weight, Tensor z, Tensor? z_aux=None, str activation='silu') -> Tensor[]");
     m.def("activation_pack8(Tensor x) -> Tensor[]");
     m.def("activation_unpack8(Tensor codes, Tensor exponents, ScalarType dtype) -> Tensor");
 }

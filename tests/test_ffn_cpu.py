@@ -127,9 +127,12 @@ def test_gated_linear_refusals():
             run(**kw)
     z = torch.zeros(6, 20, dtype=torch.bfloat16)
     do = torch.zeros(6, 10, dtype=torch.bfloat16)
-    for args, text in (((do[:5], x, w, z), "d_out must have"), ((do.float(), x, w, z), "d_out must have"), ((do, x, w, z[:5]), "z must hold"),
-                       ((do, x, w, z.to(torch.float8_e4m3fn)), "z must hold"), ((do, x, w, z, torch.zeros(6, 2, 1, dtype=torch.uint8)), "z must hold"),
-                       ((do, x, w, z.to(torch.float8_e4m3fn), torch.zeros(6, 1, dtype=torch.uint8)), "z_exponents must be"), ((do, x, w, z), "no CPU implementation")):
+    for args, text in (((do[:5], x, w, z), "d_out must have"), ((do.float(), x, w, z), "d_out must have"), ((do, x, w, z[:5]), "z must be"),
+                       ((do, x, w, z.float()), "z must be"), ((do, x, w, z), "z_aux must be"), ((do, x, w, z, torch.zeros(6, 2, 1, dtype=torch.uint8)), "z_aux must be"),
+                       ((do, x, w, z, torch.zeros(6, 20)), "z_aux must be"), ((do, x, w, z.to(torch.float8_e4m3fn), torch.zeros(6, 1, dtype=torch.uint8)), "z_aux must be"),
+                       ((do, x, w, z, torch.zeros(6, 20, dtype=torch.uint8)), "no CPU implementation"),
+                       ((do, x, w, z.to(torch.float8_e4m3fn), torch.zeros(6, 2, 1, dtype=torch.uint8)), "no CPU implementation"),
+                       ((do.float(), x.float(), w.float(), z.float()), "no CPU implementation")):
         with pytest.raises(RuntimeError, match=text):
             M.gated_linear_backward(*args)
 
@@ -201,8 +204,8 @@ def test_c_abi_gated_linear():
     for over, rc, text in ((dict(struct_size=3), -1, "size mismatch"), (dict(dtype=3), -1, "dtype expect"), (dict(bias_dtype=_capi.HSTU_F16), -1, "bias_dtype expect"),
                            (dict(act=2), -1, "act expect"), (dict(keep=3), -1, "keep expect"), (dict(keep=2, dtype=0, bias_dtype=0), -1, "8-bit checkpoints need"),
                            (dict(m=-1), -1, "x dim0"), (dict(k=0), -1, "x dim1"), (dict(k=16385), -1, "x dim1"), (dict(f=0), -1, "weight dim0"), (dict(f=32769), -1, "weight dim0"),
-                           (dict(x_stride=-1), -1, "x_stride"), (dict(x=None), -1, "must not be NULL"), (dict(z=None), -1, "z (and z_exponents"),
-                           (dict(keep=2, z_exponents=None), -1, "z (and z_exponents"), (dict(out=0x10001), -2, "aligned"), (dict(m=0, x=None), 0, "")):
+                           (dict(x_stride=-1), -1, "x_stride"), (dict(x=None), -1, "must not be NULL"), (dict(z=None), -1, "z (and z_aux"),
+                           (dict(keep=2, z_aux=None), -1, "z (and z_aux"), (dict(z_aux=None), -1, "z (and z_aux"), (dict(out=0x10001), -2, "aligned"), (dict(m=0, x=None), 0, "")):
         p = _fill(P, **over)
         assert L.hstu_hip_gated_linear_get_workspace_size(C.byref(p), C.byref(n)) == rc and (rc == 0 or text in _err()), (over, _err())
         assert L.hstu_hip_gated_linear(C.byref(p), 0x10000, 1 << 40, None) == rc

@@ -5,7 +5,8 @@ Tolerances (u = half a step of the I/O type: bf16 2^-8, fp16 2^-11, fp32 2^-24; 
 * a result is rounded once: u |result|
 * an fp32 sum of n terms is off by at most (n + 4) eps times the sum of the terms' magnitudes (any order; the 4 stands for the
   rounding of each term); where n is long the kernels add in trees of at most 64 + n / 64 steps, which `depth` says
-* dz is rounded to the I/O type before the two products: u |dz| per term of their sums
+* z is kept in 24 bits (2^-15 of the value cut off) or fp32; dz is rounded to the I/O type before the two products: u |dz| per
+  term of their sums
 * exponential, reciprocal, erfc: a few steps of fp32 each, and the rounding of their argument: (4 + |z|) eps of the value for SiLU
   and (8 + z^2) eps for GELU; both under TRANS = 2^-18 for the |z| < 40 of these inputs
 """
@@ -225,7 +226,17 @@ def gl_backward_tol(do, x, w, z, act, dtype, gtype, dz):
     return t_x, t_w, t_b
 
 
-SIZES = [(1, 1, 1), (1, 64, 32), (1, 512, 640), (2, 8, 5), (3, 37, 33), (5, 1000, 77), (16, 128, 256), (17, 130, 100), (33, 72, 129), (48, 256, 512), (64, 64, 64),
+def joined(z, aux):
+    """z as the forward keeps it: fp32, or the upper 16 and the next 8 bits of the fp32 values (cut off: 2^-15 of the value)."""
+    if z.dtype == F32:
+        return z.cpu()
+    up, low = z.cpu().view(torch.int16).to(torch.int64) & 0xffff, aux.cpu().to(torch.int64)
+    return (((up << 16) | (low << 8)) & 0xffffffff).to(torch.int64).where(up < 0x8000, (((up << 16) | (low << 8)) - (1 << 32))).to(torch.int32).view(F32)
+
+
+CUT = {F32: 0.0, HF: 2.0 ** -15, BF: 2.0 ** -15}
+
+SIZES = [(1, 1, 1), (1, 64, 32), (1, 512, 640), (2, 8, 5), (3, 37, 33), (5, 1000, 77), (16, 128, 256), (17, 130, 100), (33, 72, 129), (48, 256, 512), (64, 64, 64), (40, 40, 16400),
          (65, 16, 128), (100, 257, 31), (127, 129, 127), (130, 66, 300), (255, 96, 128), (257, 640, 200), (300, 512, 160)]
 
 
@@ -237,13 +248,14 @@ def test_gated_linear_sizes(m, k, f, dtype):
         x, w, b, do = gl_case(m, k, f, dtype, bias, 7 * m + k + f)
         out0, z0 = FO.gated_linear(x, w, b, act)
         tz, to = gl_forward_tol(x, w, b, z0, act, dtype)
-        out, z = M.gated_linear_forward(x.cuda(), w.cuda(), cu(b), act)
+        out, z, *aux = M.gated_linear_forward(x.cuda(), w.cuda(), cu(b), act)
         within(out, out0, to, "out")
-        within(z, z0, tz + U[dtype] * z0.abs() + TINY[dtype], "z")
-        assert torch.equal(M.gated_linear(x.cuda(), w.cuda(), cu(b), act), out)
+        assert z.shape == (m, 2 * f) and z.dtype == (F32 if dtype == F32 else BF) and len(aux) == (0 if dtype == F32 else 1)
         # the backward for the z that the forward kept
-        zk = z.cpu()
-        got = M.gated_linear_backward(do.cuda(), x.cuda(), w.cuda(), z, None, act)
+        zk = joined(z, *aux, *([None] if not aux else []))
+        within(zk, z0, tz + (U[F32] + CUT[dtype]) * z0.abs() + TINY[F32], "z")
+        assert torch.equal(M.gated_linear(x.cuda(), w.cuda(), cu(b), act), out)
+        got = M.gated_linear_backward(do.cuda(), x.cuda(), w.cuda(), z, *aux, activation=act)
         *want, dz = FO.gated_linear_backward(do, x, w, zk, act)
         assert got[0].dtype == got[1].dtype == dtype and got[2].dtype == F32
         for a, r, t, n in zip(got, want, gl_backward_tol(do, x, w, zk, act, dtype, dtype, dz), ("d_x", "d_weight", "d_bias")):
@@ -264,7 +276,8 @@ def test_gated_linear_larger_and_reproducible(m, k, f, dtype, act):
         runs.append([out.detach()] + list(torch.autograd.grad(out, leaves, do.cuda())))
     assert all(torch.equal(p, q) for p, q in zip(*runs))
     within(runs[0][0], out0, to, "out")
-    z = M.gated_linear_forward(x.cuda(), w.cuda(), b.cuda(), act)[1].cpu()
+    kept = M.gated_linear_forward(x.cuda(), w.cuda(), b.cuda(), act)[1:]
+    z = joined(kept[0], kept[-1])
     *want, dz = FO.gated_linear_backward(do, x, w, z, act)
     tols = list(gl_backward_tol(do, x, w, z, act, dtype, dtype, dz))
     tols[2] = tols[2] + U[dtype] * want[2].abs() + TINY[dtype]
@@ -379,18 +392,19 @@ def test_gated_linear_outputs_end_where_they_should():
         x, w, b, do = gl_case(m, k, f, dtype, True, 31)
         X, W, B, D = x.cuda(), w.cuda(), b.cuda(), do.cuda()
         mark = 123.0
-        bufs = {n: torch.full((s + 2 * 512,), mark, dtype=dtype, device="cuda") for n, s in
-                (("out", m * f), ("z", m * 2 * f), ("d_x", m * k), ("d_weight", 2 * f * k), ("d_bias", 2 * f))}
+        bufs = {n: torch.full((s + 2 * 512,), mark, dtype=t, device="cuda") for n, s, t in
+                (("out", m * f, dtype), ("z", m * 2 * f, dtype), ("z_aux", m * 2 * f, torch.uint8), ("d_x", m * k, dtype), ("d_weight", 2 * f * k, dtype),
+                 ("d_bias", 2 * f, dtype))}
         at = {n: t.data_ptr() + 512 * t.element_size() for n, t in bufs.items()}
         p = _capi.HstuGatedParams(struct_size=C.sizeof(_capi.HstuGatedParams), dtype=code, bias_dtype=code, act=0, keep=1, k=k, f=f, m=m, x_stride=k,
-                                  x=X.data_ptr(), weight=W.data_ptr(), bias=B.data_ptr(), out=at["out"], z=at["z"])
+                                  x=X.data_ptr(), weight=W.data_ptr(), bias=B.data_ptr(), out=at["out"], z=at["z"], z_aux=at["z_aux"])
         n = C.c_uint64(0)
         assert L.hstu_hip_gated_linear_get_workspace_size(C.byref(p), C.byref(n)) == 0
         ws = torch.full((n.value + 4096,), 77, dtype=torch.uint8, device="cuda")
         st = C.c_void_p(torch.cuda.current_stream().cuda_stream)
         assert L.hstu_hip_gated_linear(C.byref(p), ws.data_ptr(), n.value, st) == 0
         q = _capi.HstuGatedBwdParams(struct_size=C.sizeof(_capi.HstuGatedBwdParams), dtype=code, grad_bias_dtype=code, act=0, keep=1, k=k, f=f, m=m, x_stride=k,
-                                     dout_stride=f, d_out=D.data_ptr(), x=X.data_ptr(), weight=W.data_ptr(), z=at["z"], d_x=at["d_x"], d_weight=at["d_weight"],
+                                     dout_stride=f, d_out=D.data_ptr(), x=X.data_ptr(), weight=W.data_ptr(), z=at["z"], z_aux=at["z_aux"], d_x=at["d_x"], d_weight=at["d_weight"],
                                      d_bias=at["d_bias"])
         n2 = C.c_uint64(0)
         assert L.hstu_hip_gated_linear_backward_get_workspace_size(C.byref(q), C.byref(n2)) == 0
@@ -532,7 +546,8 @@ def test_checkpoints_hold_less_memory():
         held[c8] = torch.cuda.memory_allocated() - before - y.numel() * 2
         del y
     z = tokens * 2 * f
-    assert z * 2 <= held[False] < z * 2 + 4096 and z * 33 // 32 <= held[True] < z * 33 // 32 + 4096
+    # 24 bits, and 8 with an exponent for 32
+    assert z * 3 <= held[False] < z * 3 + 4096 and z * 33 // 32 <= held[True] < z * 33 // 32 + 4096
 
 
 def test_streams_and_graphs():
@@ -547,7 +562,7 @@ def test_streams_and_graphs():
     def step(x, c8):
         n, mean, rstd = M.layer_norm_forward(x, p["nw"], p["nb"], EPS)
         kept = M.gated_linear_forward(n, p["w"], p["b"], "silu", c8)
-        d = M.gated_linear_backward(dy, n, p["w"], kept[1], kept[2] if c8 else None, "silu")
+        d = M.gated_linear_backward(dy, n, p["w"], kept[1], kept[2], "silu")
         e = M.layer_norm_backward(d[0], x, p["nw"], mean, rstd)
         return [kept[0], *d, *e]
 
@@ -585,8 +600,8 @@ def test_two_host_threads():
     import threading
     x, w, b, do = gl_case(300, 96, 140, BF, True, 51)
     X, W, B, D = x.cuda(), w.cuda(), b.cuda(), do.cuda()
-    _, z = M.gated_linear_forward(X, W, B)
-    want = [t.clone() for t in M.gated_linear_backward(D, X, W, z)]
+    _, *z = M.gated_linear_forward(X, W, B)
+    want = [t.clone() for t in M.gated_linear_backward(D, X, W, *z)]
     torch.cuda.synchronize()
     bad = []
 
@@ -594,7 +609,7 @@ def test_two_host_threads():
         s = torch.cuda.Stream()
         with torch.cuda.stream(s):
             for _ in range(20):
-                got = M.gated_linear_backward(D, X, W, z)
+                got = M.gated_linear_backward(D, X, W, *z)
                 s.synchronize()
                 if not all(torch.equal(a, c) for a, c in zip(got, want)):
                     bad.append(1)
