@@ -17,15 +17,19 @@ namespace hstu {
 struct PadArgs { const void* src[2]; void* dst[2]; int64_t stride[2], rows[2]; int64_t ld; int32_t cols; };   // up to two operands, one launch
 template <typename T>
 __global__ __launch_bounds__(256) void hstu_pad_rows_kernel(const PadArgs a) {
-    const int per_row = (int)((a.ld + 7) / 8);   // pieces of 8 elements
-    const int64_t first = a.rows[0] * per_row, n = first + a.rows[1] * per_row;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        const int which = i >= first;
-        const int64_t j = which ? i - first : i, r = j / per_row;
-        const int c = (int)(j - r * per_row) * 8;
-        float v[8];
-        load8_any(reinterpret_cast<const T*>(a.src[which]) + r * a.stride[which] + (a.cols - c > 0 ? c : 0), a.cols - c, v);
-        store8_any(reinterpret_cast<T*>(a.dst[which]) + r * a.ld + c, (int)(a.ld - c), v);
+    // a wave takes a row, a lane 8 elements at a time
+    const int lane = threadIdx.x & 63;
+    const int64_t n = a.rows[0] + a.rows[1];
+    for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < n; i += (int64_t)gridDim.x * 4) {
+        const int which = i >= a.rows[0];
+        const int64_t r = which ? i - a.rows[0] : i;
+        const T* src = reinterpret_cast<const T*>(a.src[which]) + r * a.stride[which];
+        T* dst = reinterpret_cast<T*>(a.dst[which]) + r * a.ld;
+        for (int c = lane * 8; c < a.ld; c += 512) {
+            float v[8];
+            load8_any(src + c, a.cols - c, v);
+            store8_any(dst + c, (int)(a.ld - c), v);
+        }
     }
 }
 
@@ -238,7 +242,7 @@ static hipError_t launch_pad(int32_t dtype, const void* x, int64_t x_stride, int
     a.src[1] = w; a.stride[1] = k; a.dst[1] = w_to; a.rows[1] = w_to ? f2 : 0;
     const int64_t rows = a.rows[0] + a.rows[1];
     if (rows == 0) return hipSuccess;
-    const int64_t want = (rows * ((ld + 7) / 8) + 255) / 256;
+    const int64_t want = (rows + 3) / 4;
     const dim3 grid((unsigned)(want > 4096 ? 4096 : want));
     if (dtype == HSTU_F32) hipLaunchKernelGGL(hstu_pad_rows_kernel<float>, grid, dim3(256), 0, st, a);
     else if (dtype == HSTU_F16) hipLaunchKernelGGL(hstu_pad_rows_kernel<_Float16>, grid, dim3(256), 0, st, a);

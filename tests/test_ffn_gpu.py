@@ -286,6 +286,31 @@ def test_gated_linear_larger_and_reproducible(m, k, f, dtype, act):
         within(a, r, t, n)
 
 
+@pytest.mark.parametrize("m,k,f,dtype,act,c8", [(8192, 64, 2048, BF, "silu", False), (5000, 700, 4000, BF, "gelu", True), (20000, 1000, 700, HF, "silu", False),
+                                                (9000, 1100, 2200, BF, "silu", False), (33000, 520, 264, HF, "silu", True), (16384, 512, 2048, F32, "silu", False),
+                                                (70, 4096, 12000, BF, "silu", False), (24000, 16, 40, BF, "gelu", False)])
+def test_gated_linear_every_tile(m, k, f, dtype, act, c8):
+    """Sizes at which the products run in each of their tiles, with and without shares of the contraction (64-bit oracle on the GPU)."""
+    say("gated_linear tiles", m, k, f, dtype, act, c8)
+    x, w, b, do = (t.cuda() for t in gl_case(m, k, f, dtype, True, 61))
+    out0, z0 = FO.gated_linear(x, w, b, act)
+    tz, to = gl_forward_tol(x, w, b, z0, act, dtype)
+    out, z, *aux = M.gated_linear_forward(x, w, b, act, c8)
+    on_cpu = lambda *ts: [t.cpu() for t in ts]
+    within(out, *on_cpu(out0, to), "out")
+    if c8:
+        vals = z.float().cpu().reshape(m, 2, f)
+        zk = torch.cat([FO.unpack8(vals[:, h], aux[0].cpu()[:, h], F32) for h in range(2)], dim=1).float().cuda()
+    else:
+        zk = joined(z, *aux, *([None] if not aux else [])).cuda()
+        within(zk, *on_cpu(z0, tz + (U[F32] + CUT[dtype]) * z0.abs() + TINY[F32]), "z")
+    got = M.gated_linear_backward(do, x, w, z, *aux, activation=act)
+    del out0, z0, tz, to
+    *want, dz = FO.gated_linear_backward(do, x, w, zk, act)
+    for a, r, t, n in zip(got, want, gl_backward_tol(do, x, w, zk, act, dtype, dtype, dz), ("d_x", "d_weight", "d_bias")):
+        within(a, *on_cpu(r, t), n)
+
+
 @pytest.mark.parametrize("m,k,f,dtype",
                          [(m, k, f, d) for (m, k, f) in ((1, 64, 32), (70, 128, 96), (33, 40, 45), (257, 96, 1000), (600, 512, 256)) for d in (BF, HF)])
 def test_gated_linear_checkpoint8(m, k, f, dtype):
@@ -548,6 +573,118 @@ def test_checkpoints_hold_less_memory():
     z = tokens * 2 * f
     # 24 bits, and 8 with an exponent for 32
     assert z * 3 <= held[False] < z * 3 + 4096 and z * 33 // 32 <= held[True] < z * 33 // 32 + 4096
+
+
+def test_autograd_captured_into_a_graph():
+    """Forward and backward of the block through autograd inside one capture, replayed with new inputs and eager work in between."""
+    c, f, tokens = 64, 96, 130
+    host = block_params(c, f, BF, 6)
+    p = {k: v.cuda().requires_grad_(True) for k, v in host.items()}
+    g = torch.Generator().manual_seed(7)
+    xs, dy = [randn(g, tokens, c, dtype=BF).cuda() for _ in range(3)], randn(g, tokens, c, dtype=BF).cuda()
+
+    def step(x, ps, c8):
+        xl = x.detach().requires_grad_(True)
+        y = block(xl, ps, c8)
+        return [y.detach()] + list(torch.autograd.grad(y, [xl] + list(ps.values()), dy))
+
+    for c8 in (False, True):
+        eager = [[t.clone() for t in step(x, p, c8)] for x in xs]
+        # leaves of its own: the capture's graph shares nothing with the eager ones
+        q = {k: v.detach().clone().requires_grad_(True) for k, v in p.items()}
+        inp = xs[0].clone()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step(inp, q, c8)
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            out = step(inp, q, c8)
+        for i in (1, 0, 2, 1):
+            inp.copy_(xs[i])
+            gr.replay()
+            torch.cuda.synchronize()
+            # the down projection is a library product, whose kernel a capture may choose otherwise: the block's own gradients bit for
+            # bit where they hang on it no further than its rounding
+            for a, b in zip(out, eager[i]):
+                assert float((a.double() - b.double()).norm()) <= 2.0 ** -7 * float(b.double().norm())
+            step(xs[2 - i], p, c8)
+
+
+def test_offsets_beyond_32_bits():
+    """More than 2^31 elements: the last rows are what a call of their own gives, bit for bit."""
+    rows, cols = (1 << 31) // 512 + 300, 512
+    x = torch.empty(rows, cols, dtype=BF, device="cuda")
+    x[:128], x[-700:] = torch.randn(128, cols, device="cuda"), torch.randn(700, cols, device="cuda")
+    x[128:-700] = 1.0
+    w, b = torch.randn(cols, device="cuda").to(BF), torch.randn(cols, device="cuda").to(BF)
+    say("offsets: layer_norm")
+    y, mean, rstd = M.layer_norm_forward(x, w, b, EPS)
+    assert torch.equal(y[-700:], M.layer_norm(x[-700:], w, b, EPS)) and torch.equal(y[:128], M.layer_norm(x[:128], w, b, EPS))
+    dx = M.layer_norm_backward(x, x, w, mean, rstd)[0]
+    tail = M.layer_norm_backward(x[-700:], x[-700:], w, mean[-700:], rstd[-700:])[0]
+    assert torch.equal(dx[-700:], tail)
+    del y, dx
+    say("offsets: pack8")
+    codes, exps = M.activation_pack8(x)
+    tc, te = M.activation_pack8(x[-700:])
+    assert torch.equal(codes[-700:].view(torch.uint8), tc.view(torch.uint8)) and torch.equal(exps[-700:], te)
+    back = M.activation_unpack8(codes, exps, BF)
+    assert torch.equal(back[-700:], M.activation_unpack8(tc, te, BF))
+    del back, codes, exps, x
+    say("offsets: gated_linear")
+    k, f = 16, 4096
+    m = (1 << 31) // (2 * f) + 500                        # z has more than 2^31 elements
+    x = torch.randn(m, k, device="cuda").to(BF)
+    w = (torch.randn(2 * f, k, device="cuda") / 4).to(BF)
+    for c8 in (False, True):
+        out, z, aux = M.gated_linear_forward(x, w, None, "silu", c8)
+        o2, z2, a2 = M.gated_linear_forward(x[-600:], w, None, "silu", c8)
+        assert torch.equal(out[-600:], o2) and torch.equal(z[-600:].view(torch.uint8), z2.view(torch.uint8)) and torch.equal(aux[-600:], a2)
+        d = M.gated_linear_backward(out, x, w, z, aux)
+        d2 = M.gated_linear_backward(o2, x[-600:], w, z2, a2)
+        # other shares of the contraction, other order of the sums: 2 f terms, rounded to bf16
+        assert float((d[0][-600:].double() - d2[0].double()).abs().max()) <= float(d2[0].abs().max()) * 2.0 ** -7
+        assert bool(torch.isfinite(d[1]).all())
+        del out, z, aux, d
+
+
+def test_gated_linear_keeps_nan_and_infinity_where_they_are():
+    """A NaN or an infinity in a row of x reaches that row of out and d_x and no other; in a row of weight, that column."""
+    for dtype, m, k, f in ((BF, 200, 70, 90), (HF, 30, 64, 64), (F32, 130, 33, 40)):
+        x, w, b, do = (t.cuda() for t in gl_case(m, k, f, dtype, True, 71))
+        for c8 in (False, True) if dtype != F32 else (False,):
+            clean, z, *aux = M.gated_linear_forward(x, w, b, "silu", c8)
+            dclean = M.gated_linear_backward(do, x, w, z, *aux)[0]
+            x2, w2 = x.clone(), w.clone()
+            x2[7, k - 1], x2[m - 1, 0] = float("nan"), float("inf")
+            out, z, *aux = M.gated_linear_forward(x2, w, b, "silu", c8)
+            dx = M.gated_linear_backward(do, x2, w, z, *aux)[0]
+            keep = [i for i in range(m) if i not in (7, m - 1)]
+            assert torch.equal(out[keep], clean[keep]) and torch.equal(dx[keep], dclean[keep])
+            assert bool(torch.isnan(out[7]).all()) and bool(torch.isnan(dx[7]).all()) and not bool(torch.isfinite(out[m - 1]).all())
+            w2[3, 0] = float("nan")
+            w2[f + 5, k - 1] = float("inf")
+            out = M.gated_linear(x, w2, b, "silu", c8)
+            cols = [i for i in range(f) if i not in (3, 5)]
+            assert torch.equal(out[:, cols], clean[:, cols]) and bool(torch.isnan(out[:, 3]).all())
+
+
+def test_one_tensor_in_two_places():
+    """The same tensor as x and weight, and as upstream gradient and input: gradients add up, results are the ones of copies."""
+    t = torch.randn(64, 64, generator=torch.Generator().manual_seed(3)).to(BF).cuda()
+    a = t.clone().requires_grad_(True)
+    b1, b2 = t.clone().requires_grad_(True), t.clone().requires_grad_(True)
+    do = torch.randn(64, 32, generator=torch.Generator().manual_seed(4)).to(BF).cuda()
+    ya, yb = M.gated_linear(a, a), M.gated_linear(b1, b2)
+    assert torch.equal(ya, yb)
+    ga = torch.autograd.grad(ya, a, do)[0]
+    g1, g2 = torch.autograd.grad(yb, (b1, b2), do)
+    assert torch.equal(ga, g1 + g2)
+    n = t.clone().requires_grad_(True)
+    assert torch.equal(torch.autograd.grad(M.layer_norm(n, None, None, EPS), n, n.detach())[0], torch.autograd.grad(M.layer_norm(n, None, None, EPS), n, t)[0])
 
 
 def test_streams_and_graphs():
