@@ -94,10 +94,12 @@ int hstu_hip_activation_unpack8(const hstu_pack8_params* p, void* stream);
  *   out = round(act(z[:, :f]) * z[:, f:])
  * keep says what the backward gets: nothing, z, or z in 8 bits.  z is kept in fp32 for HSTU_F32 and in 24 bits otherwise: the upper
  * 16 bits of the fp32 value in z, the next 8 in z_aux (1 + 8 + 15 bits; rounded to 16 bits, z alone would put as large an error into
- * the gradients as the rounding of dz and of the gradients themselves).  In 8 bits the groups of the two halves do not mix: the
- * exponents in z_aux are [m, 2, ceil(f / 32)].  m may be 0. */
+ * the gradients as the rounding of dz and of the gradients themselves).  What is kept has rows of 2 fp columns, fp = f rounded up to
+ * a multiple of 32 (HSTU_GATED_KEPT(f)): the gate's f, zeros, the values' f, zeros; in 8 bits z_aux has an exponent for each 32 of
+ * them, [m, 2, fp / 32].  m may be 0. */
 #define HSTU_GATED_MAX_K 16384
 #define HSTU_GATED_MAX_F 32768
+#define HSTU_GATED_KEPT(f) (((f) + 31) / 32 * 32)
 enum { HSTU_ACT_SILU = 0, HSTU_ACT_GELU = 1 /* z * Phi(z), with erf */ };
 enum { HSTU_KEEP_NONE = 0, HSTU_KEEP_FULL = 1, HSTU_KEEP_8BIT = 2 /* 16-bit dtypes only */ };
 typedef struct hstu_gated_params {
@@ -115,8 +117,8 @@ typedef struct hstu_gated_params {
     const void* weight;    /* [2 f, k], contiguous */
     const void* bias;      /* [2 f], or NULL */
     void* out;             /* [m, f], contiguous */
-    void* z;               /* HSTU_KEEP_FULL: [m, 2 f] fp32 or 16-bit upper parts; HSTU_KEEP_8BIT: codes [m, 2 f] */
-    uint8_t* z_aux;        /* HSTU_KEEP_FULL of 16-bit dtypes: lower parts [m, 2 f]; HSTU_KEEP_8BIT: exponents */
+    void* z;               /* HSTU_KEEP_FULL: [m, 2, fp] fp32 or 16-bit upper parts; HSTU_KEEP_8BIT: codes [m, 2, fp] */
+    uint8_t* z_aux;        /* HSTU_KEEP_FULL of 16-bit dtypes: lower parts [m, 2, fp]; HSTU_KEEP_8BIT: exponents */
 } hstu_gated_params;
 int hstu_hip_gated_linear_get_workspace_size(const hstu_gated_params* p, uint64_t* workspace_bytes);
 int hstu_hip_gated_linear(const hstu_gated_params* p, void* workspace, uint64_t workspace_bytes, void* stream);

@@ -55,7 +55,7 @@ __global__ __launch_bounds__(256) void hstu_gated_dz_kernel(const DzArgs a) {
     const int64_t rb = blockIdx.x / a.col_blocks;
     const int c = (cb * lanes + tx) * 8, n = a.f - c;
     const int64_t r0 = rb * a.rows_wg, r1 = min(r0 + a.rows_wg, a.m);
-    const int groups = (a.f + HSTU_PACK8_GROUP - 1) / HSTU_PACK8_GROUP;
+    const int64_t kept = HSTU_GATED_KEPT((int64_t)a.f);
     float sg[8], su[8];
 #pragma unroll
     for (int k = 0; k < 8; k++) sg[k] = su[k] = 0.f;
@@ -64,19 +64,19 @@ __global__ __launch_bounds__(256) void hstu_gated_dz_kernel(const DzArgs a) {
             float d[8], zg[8], zu[8];
             load8_any(reinterpret_cast<const T*>(a.d_out) + r * a.dout_stride + c, n, d);
             if (a.keep == HSTU_KEEP_8BIT) {
-                const uint8_t* z = reinterpret_cast<const uint8_t*>(a.z) + r * 2 * a.f + c;
-                const uint8_t* e = a.z_aux + r * 2 * groups + c / HSTU_PACK8_GROUP;
-                code_values(codes8_raw(z, n, e[0]), largest_finite<float>(), zg);
-                code_values(codes8_raw(z + a.f, n, e[groups]), largest_finite<float>(), zu);
+                const uint8_t* z = reinterpret_cast<const uint8_t*>(a.z) + r * 2 * kept + c;
+                const uint8_t* e = a.z_aux + (r * 2 * kept + c) / HSTU_PACK8_GROUP;
+                code_values(codes8_raw(z, 8, e[0]), largest_finite<float>(), zg);
+                code_values(codes8_raw(z + kept, 8, e[kept / HSTU_PACK8_GROUP]), largest_finite<float>(), zu);
             } else if constexpr (sizeof(T) == 4) {
-                const T* z = reinterpret_cast<const T*>(a.z) + r * 2 * a.f + c;
-                load8_any(z, n, zg);
-                load8_any(z + a.f, n, zu);
+                const T* z = reinterpret_cast<const T*>(a.z) + r * 2 * kept + c;
+                load8_any(z, 8, zg);
+                load8_any(z + kept, 8, zu);
             } else {
-                const T* z = reinterpret_cast<const T*>(a.z) + r * 2 * a.f + c;
-                const uint8_t* low = a.z_aux + r * 2 * a.f + c;
-                const Raw8<T> ug = load8_raw(z, n), uu = load8_raw(z + a.f, n);
-                const Codes8 lg = codes8_raw(low, n, 0), lu = codes8_raw(low + a.f, n, 0);
+                const T* z = reinterpret_cast<const T*>(a.z) + r * 2 * kept + c;
+                const uint8_t* low = a.z_aux + r * 2 * kept + c;
+                const Raw8<T> ug = load8_raw(z, 8), uu = load8_raw(z + kept, 8);
+                const Codes8 lg = codes8_raw(low, 8, 0), lu = codes8_raw(low + kept, 8, 0);
                 join24(ug.q[0], lg.q, zg);
                 join24(uu.q[0], lu.q, zu);
             }

@@ -70,18 +70,9 @@ __global__ __launch_bounds__(64 * ROWS_WAVES) void hstu_gated_rows_kernel(const 
         for (int b = 0; b < FB; b++)
 #pragma unroll
             for (int j = 0; j < MB; j++) acc[h][b][j] = gm_f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int k0 = w * PIECE; k0 < a.k; k0 += W * PIECE) {
-        frag wf[2][2][FB], xf[2][MB];
-#pragma unroll
-        for (int s = 0; s < 2; s++) {
-            const int at = k0 + 4 * EC * s, n = a.k - (at + q * EC), o = n > 0 ? at : 0;
-#pragma unroll
-            for (int h = 0; h < 2; h++)
-#pragma unroll
-                for (int b = 0; b < FB; b++) wf[s][h][b] = load_frag(wrow[h][b] + o, n);
-#pragma unroll
-            for (int j = 0; j < MB; j++) xf[s][j] = load_frag(xrow[j] + o, n);
-        }
+    // whole pieces without a branch between their loads; only a row's last piece may be shorter
+    struct Piece { frag w[2][2][FB], x[2][MB]; };
+    auto multiply = [&](const Piece& p) __attribute__((always_inline)) {
 #pragma unroll
         for (int s = 0; s < 2; s++)
 #pragma unroll
@@ -89,7 +80,37 @@ __global__ __launch_bounds__(64 * ROWS_WAVES) void hstu_gated_rows_kernel(const 
 #pragma unroll
                 for (int b = 0; b < FB; b++)
 #pragma unroll
-                    for (int j = 0; j < MB; j++) acc[h][b][j] = mfma16(wf[s][h][b], xf[s][j], acc[h][b][j]);
+                    for (int j = 0; j < MB; j++) acc[h][b][j] = mfma16(p.w[s][h][b], p.x[s][j], acc[h][b][j]);
+    };
+    int k0 = w * PIECE;
+#pragma unroll 2
+    for (; k0 + PIECE <= a.k; k0 += W * PIECE) {
+        Piece p;
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            const int at = k0 + 4 * EC * s;
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int b = 0; b < FB; b++) p.w[s][h][b] = __builtin_bit_cast(frag, *reinterpret_cast<const gm_u4_any*>(wrow[h][b] + at));
+#pragma unroll
+            for (int j = 0; j < MB; j++) p.x[s][j] = __builtin_bit_cast(frag, *reinterpret_cast<const gm_u4_any*>(xrow[j] + at));
+        }
+        multiply(p);
+    }
+    if (k0 < a.k) {
+        Piece p;
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            const int at = k0 + 4 * EC * s, n = a.k - (at + q * EC), o = n > 0 ? at : 0;
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int b = 0; b < FB; b++) p.w[s][h][b] = load_frag(wrow[h][b] + o, n);
+#pragma unroll
+            for (int j = 0; j < MB; j++) p.x[s][j] = load_frag(xrow[j] + o, n);
+        }
+        multiply(p);
     }
     // a lane holds f = 16 b + 4 q + e of row m = 16 j + r16
 #pragma unroll
@@ -120,20 +141,20 @@ __global__ __launch_bounds__(64 * ROWS_WAVES) void hstu_gated_rows_kernel(const 
     __syncthreads();
     for (int v = threadIdx.x; v < a.m * 16 * FB; v += 64 * W) {
         const int m = v / (16 * FB), c = v % (16 * FB), f = f0 + c;
-        if (f >= a.f) continue;
         const float zg = zs[0][m][c], zu = zs[1][m][c];
-        reinterpret_cast<T*>(a.out)[(int64_t)m * a.f + f] = from_float<T>(act_of(zg, a.act) * zu);
+        if (f < a.f) reinterpret_cast<T*>(a.out)[(int64_t)m * a.f + f] = from_float<T>(act_of(zg, a.act) * zu);
         if (a.keep == HSTU_KEEP_FULL) {
-            const int64_t at = (int64_t)m * 2 * a.f + f;
+            const int kept = HSTU_GATED_KEPT(a.f);   // (the grid covers the kept columns, and only those)
+            const int64_t at = (int64_t)m * 2 * kept + f;
             if constexpr (sizeof(T) == 4) {
                 reinterpret_cast<T*>(a.z)[at] = zg;
-                reinterpret_cast<T*>(a.z)[at + a.f] = zu;
+                reinterpret_cast<T*>(a.z)[at + kept] = zu;
             } else {
                 const unsigned bg = __builtin_bit_cast(unsigned, zg), bu = __builtin_bit_cast(unsigned, zu);
                 reinterpret_cast<uint16_t*>(a.z)[at] = (uint16_t)(bg >> 16);
-                reinterpret_cast<uint16_t*>(a.z)[at + a.f] = (uint16_t)(bu >> 16);
+                reinterpret_cast<uint16_t*>(a.z)[at + kept] = (uint16_t)(bu >> 16);
                 a.z_aux[at] = (uint8_t)(bg >> 8);
-                a.z_aux[at + a.f] = (uint8_t)(bu >> 8);
+                a.z_aux[at + kept] = (uint8_t)(bu >> 8);
             }
         }
     }
@@ -144,14 +165,13 @@ __global__ __launch_bounds__(64 * ROWS_WAVES) void hstu_gated_rows_kernel(const 
             for (int c = 0; c < 32; c++) top = fmaxf(top, pack8_finite_abs(zs[h][m][c]));
             const int e = pack8_exponent(top);
             const float inv = pack8_inv_scale(e);
-            const int groups = (a.f + HSTU_PACK8_GROUP - 1) / HSTU_PACK8_GROUP;
-            a.z_aux[((int64_t)m * 2 + h) * groups + blockIdx.x] = (uint8_t)e;
-            uint8_t* z = reinterpret_cast<uint8_t*>(a.z) + ((int64_t)m * 2 + h) * a.f + f0;
+            const int64_t at = ((int64_t)m * 2 + h) * HSTU_GATED_KEPT(a.f) + f0;
+            a.z_aux[at / HSTU_PACK8_GROUP] = (uint8_t)e;
+            uint8_t* z = reinterpret_cast<uint8_t*>(a.z) + at;
             for (int c = 0; c < 32; c += 4) {
                 const unsigned u = pack8_codes(zs[h][m][c], zs[h][m][c + 1], zs[h][m][c + 2], zs[h][m][c + 3], inv);
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-                    if (f0 + c + i < a.f) z[c + i] = (uint8_t)(u >> (8 * i));
+                for (int i = 0; i < 4; i++) z[c + i] = (uint8_t)(u >> (8 * i));
             }
         }
     }
@@ -164,7 +184,8 @@ hipError_t launch_gated_rows_f32(const RowsArgs& a, hipStream_t st);
 template <typename T> hipError_t launch_gated_rows_t(const RowsArgs& a, hipStream_t st) {
     // 8-bit groups of 32 columns stay within a workgroup
     const bool wide = a.keep == HSTU_KEEP_8BIT;
-    const dim3 grid((unsigned)((a.f + (wide ? 31 : 15)) / (wide ? 32 : 16))), nt(64 * ROWS_WAVES);
+    const int cols = a.keep == HSTU_KEEP_NONE ? a.f : HSTU_GATED_KEPT(a.f);
+    const dim3 grid((unsigned)((cols + (wide ? 31 : 15)) / (wide ? 32 : 16))), nt(64 * ROWS_WAVES);
 #define GR_GO(MB)                                                                                              \
     do {                                                                                                       \
         if (wide) hipLaunchKernelGGL((hstu_gated_rows_kernel<T, MB, 2>), grid, nt, 0, st, a);                  \

@@ -376,24 +376,27 @@ __global__ __launch_bounds__(S::NT) void hstu_gemm_kernel(const GemmArgs a) {
                 h[r] = act_of(zg[r], a.act) * zu[r];
             }
             store_block<T>(reinterpret_cast<T*>(a.out) + m * a.N + n, h, g, left);
+            // kept rows are padded to whole blocks; columns past f hold zero (no weight row, no bias)
+            const int64_t kept = HSTU_GATED_KEPT((int64_t)a.N);
+            const int whole = left > 0 ? 32 : 0;
             if (a.keep == HSTU_KEEP_FULL) {
 #pragma unroll
                 for (int part = 0; part < 2; part++) {
                     const float* v = part ? zu : zg;
-                    const int64_t at = (m * 2 + part) * a.N + n;
-                    if constexpr (S::ES == 4) store_block<T>(reinterpret_cast<T*>(a.z) + at, v, g, left);
+                    const int64_t at = (m * 2 + part) * kept + n;
+                    if constexpr (S::ES == 4) store_block<T>(reinterpret_cast<T*>(a.z) + at, v, g, whole);
                     else {
                         unsigned up[8], low[4];
 #pragma unroll
                         for (int i = 0; i < 8; i++) up[i] = upper_pair(v[2 * i], v[2 * i + 1]);
 #pragma unroll
                         for (int i = 0; i < 4; i++) low[i] = lower_quad(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-                        store_pairs(reinterpret_cast<T*>(a.z) + at, up, g, left);
-                        store_quads(a.z_aux + at, low, g, left);
+                        store_pairs(reinterpret_cast<T*>(a.z) + at, up, g, whole);
+                        store_quads(a.z_aux + at, low, g, whole);
                     }
                 }
             } else if (a.keep == HSTU_KEEP_8BIT) {
-                // the 32 columns of a row lie in the 16 registers of two lanes; columns past f hold zero (no bias, no weight row)
+                // the 32 columns of a row lie in the 16 registers of two lanes
 #pragma unroll
                 for (int part = 0; part < 2; part++) {
                     const float* v = part ? zu : zg;
@@ -406,11 +409,8 @@ __global__ __launch_bounds__(S::NT) void hstu_gemm_kernel(const GemmArgs a) {
                     unsigned c[4];
 #pragma unroll
                     for (int rr = 0; rr < 4; rr++) c[rr] = pack8_codes(v[4 * rr], v[4 * rr + 1], v[4 * rr + 2], v[4 * rr + 3], inv);
-                    store_quads(reinterpret_cast<uint8_t*>(a.z) + (m * 2 + part) * a.N + n, c, g, left);
-                    if (g == 0 && left > 0) {
-                        const int groups = (a.N + HSTU_PACK8_GROUP - 1) / HSTU_PACK8_GROUP;
-                        a.z_aux[(m * 2 + part) * groups + n / HSTU_PACK8_GROUP] = (uint8_t)e;
-                    }
+                    store_quads(reinterpret_cast<uint8_t*>(a.z) + (m * 2 + part) * kept + n, c, g, whole);
+                    if (g == 0 && left > 0) a.z_aux[((m * 2 + part) * kept + n) / HSTU_PACK8_GROUP] = (uint8_t)e;
                 }
             }
         }

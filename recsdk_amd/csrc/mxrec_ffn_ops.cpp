@@ -261,11 +261,11 @@ static std::vector<at::Tensor> gl_forward(const at::Tensor& x, const at::Tensor&
     check_devices(GL, {&x, &weight, &bias});
     Launch launch(x);
     const at::Tensor xr = rows_of(x), w = weight.contiguous(), b = bias.defined() ? bias.contiguous() : bias;
-    const int64_t m = row_count(x), f = weight.size(0) / 2, groups = (f + HSTU_PACK8_GROUP - 1) / HSTU_PACK8_GROUP;
+    const int64_t m = row_count(x), f = weight.size(0) / 2, kept = HSTU_GATED_KEPT(f);
     std::vector<at::Tensor> outs{at::empty(with_last(x, f), x.options().memory_format(at::MemoryFormat::Contiguous))};
-    if (keep != HSTU_KEEP_NONE) outs.push_back(at::empty({m, 2 * f}, x.options().dtype(kept_type(x, keep == HSTU_KEEP_8BIT))));
-    if (keep == HSTU_KEEP_8BIT) outs.push_back(at::empty({m, 2, groups}, x.options().dtype(at::kByte)));
-    else if (keep == HSTU_KEEP_FULL && x.scalar_type() != at::kFloat) outs.push_back(at::empty({m, 2 * f}, x.options().dtype(at::kByte)));
+    if (keep != HSTU_KEEP_NONE) outs.push_back(at::empty({m, 2, kept}, x.options().dtype(kept_type(x, keep == HSTU_KEEP_8BIT))));
+    if (keep == HSTU_KEEP_8BIT) outs.push_back(at::empty({m, 2, kept / HSTU_PACK8_GROUP}, x.options().dtype(at::kByte)));
+    else if (keep == HSTU_KEEP_FULL && x.scalar_type() != at::kFloat) outs.push_back(at::empty({m, 2, kept}, x.options().dtype(at::kByte)));
     hstu_gated_params p;
     std::memset(&p, 0, sizeof(p));
     p.struct_size = sizeof(p);
@@ -378,11 +378,11 @@ std::vector<at::Tensor> gated_linear_backward(const at::Tensor& d_out, const at:
     const at::Tensor aux = value(z_aux);
     const bool c8 = z.scalar_type() == at::kFloat8_e4m3fn;
     gl_check(x, weight, at::Tensor(), c8);
-    const int64_t m = row_count(x), f = weight.size(0) / 2, groups = (f + HSTU_PACK8_GROUP - 1) / HSTU_PACK8_GROUP;
+    const int64_t m = row_count(x), f = weight.size(0) / 2, kept = HSTU_GATED_KEPT(f);
     TORCH_CHECK(d_out.scalar_type() == x.scalar_type() && d_out.sizes().vec() == with_last(x, f), GL, ": d_out must have the dtype of x and the shape of out");
-    TORCH_CHECK(z.numel() == m * 2 * f && z.scalar_type() == kept_type(x, c8), GL, ": z must be what gated_linear_forward kept: ", m, " x ", 2 * f,
-                " values, float32 for float32 rows, bfloat16 upper parts or float8_e4m3fn codes otherwise");
-    const int64_t want = c8 ? m * 2 * groups : x.scalar_type() == at::kFloat ? 0 : m * 2 * f;
+    TORCH_CHECK(z.numel() == m * 2 * kept && z.scalar_type() == kept_type(x, c8), GL, ": z must be what gated_linear_forward kept: [", m, ", 2, ", kept,
+                "], float32 for float32 rows, bfloat16 upper parts or float8_e4m3fn codes otherwise");
+    const int64_t want = c8 ? m * 2 * kept / HSTU_PACK8_GROUP : x.scalar_type() == at::kFloat ? 0 : m * 2 * kept;
     TORCH_CHECK(want == 0 || (aux.defined() && aux.scalar_type() == at::kByte && aux.numel() == want), GL,
                 ": z_aux must be what gated_linear_forward kept beside z: uint8, ", want, " values");
     return gl_backward(d_out, x, weight, z, want ? aux : at::Tensor(), act_code(activation), at::kFloat, true, true, true);

@@ -226,10 +226,11 @@ def gl_backward_tol(do, x, w, z, act, dtype, gtype, dz):
     return t_x, t_w, t_b
 
 
-def joined(z, aux):
+def joined(f, z, aux=None):
     """z as the forward keeps it: fp32, or the upper 16 and the next 8 bits of the fp32 values (cut off: 2^-15 of the value)."""
     if z.dtype == F32:
-        return z.cpu()
+        return z.cpu()[:, :, :f].reshape(z.shape[0], 2 * f)
+    z, aux = z[:, :, :f].reshape(z.shape[0], 2 * f).contiguous(), aux[:, :, :f].reshape(z.shape[0], 2 * f)
     up, low = z.cpu().view(torch.int16).to(torch.int64) & 0xffff, aux.cpu().to(torch.int64)
     return (((up << 16) | (low << 8)) & 0xffffffff).to(torch.int64).where(up < 0x8000, (((up << 16) | (low << 8)) - (1 << 32))).to(torch.int32).view(F32)
 
@@ -250,9 +251,10 @@ def test_gated_linear_sizes(m, k, f, dtype):
         tz, to = gl_forward_tol(x, w, b, z0, act, dtype)
         out, z, *aux = M.gated_linear_forward(x.cuda(), w.cuda(), cu(b), act)
         within(out, out0, to, "out")
-        assert z.shape == (m, 2 * f) and z.dtype == (F32 if dtype == F32 else BF) and len(aux) == (0 if dtype == F32 else 1)
+        assert z.shape == (m, 2, (f + 31) // 32 * 32) and z.dtype == (F32 if dtype == F32 else BF) and len(aux) == (0 if dtype == F32 else 1)
+        assert not bool(z[:, :, f:].float().any())                     # zeros behind the columns
         # the backward for the z that the forward kept
-        zk = joined(z, *aux, *([None] if not aux else []))
+        zk = joined(f, z, *aux)
         within(zk, z0, tz + (U[F32] + CUT[dtype]) * z0.abs() + TINY[F32], "z")
         assert torch.equal(M.gated_linear(x.cuda(), w.cuda(), cu(b), act), out)
         got = M.gated_linear_backward(do.cuda(), x.cuda(), w.cuda(), z, *aux, activation=act)
@@ -277,7 +279,7 @@ def test_gated_linear_larger_and_reproducible(m, k, f, dtype, act):
     assert all(torch.equal(p, q) for p, q in zip(*runs))
     within(runs[0][0], out0, to, "out")
     kept = M.gated_linear_forward(x.cuda(), w.cuda(), b.cuda(), act)[1:]
-    z = joined(kept[0], kept[-1])
+    z = joined(f, *kept)
     *want, dz = FO.gated_linear_backward(do, x, w, z, act)
     tols = list(gl_backward_tol(do, x, w, z, act, dtype, dtype, dz))
     tols[2] = tols[2] + U[dtype] * want[2].abs() + TINY[dtype]
@@ -299,10 +301,10 @@ def test_gated_linear_every_tile(m, k, f, dtype, act, c8):
     on_cpu = lambda *ts: [t.cpu() for t in ts]
     within(out, *on_cpu(out0, to), "out")
     if c8:
-        vals = z.float().cpu().reshape(m, 2, f)
+        vals = z.float().cpu()[:, :, :f]
         zk = torch.cat([FO.unpack8(vals[:, h], aux[0].cpu()[:, h], F32) for h in range(2)], dim=1).float().cuda()
     else:
-        zk = joined(z, *aux, *([None] if not aux else [])).cuda()
+        zk = joined(f, z, *aux).cuda()
         within(zk, *on_cpu(z0, tz + (U[F32] + CUT[dtype]) * z0.abs() + TINY[F32]), "z")
     got = M.gated_linear_backward(do, x, w, z, *aux, activation=act)
     del out0, z0, tz, to
@@ -323,9 +325,9 @@ def test_gated_linear_checkpoint8(m, k, f, dtype):
     tz, _ = gl_forward_tol(x, w, b, z0, "silu", dtype)
     out, codes, exps = M.gated_linear_forward(x.cuda(), w.cuda(), b.cuda(), "silu", True)
     groups = (f + 31) // 32
-    assert codes.shape == (m, 2 * f) and codes.dtype == torch.float8_e4m3fn and exps.shape == (m, 2, groups) and exps.dtype == torch.uint8
+    assert codes.shape == (m, 2, 32 * groups) and codes.dtype == torch.float8_e4m3fn and exps.shape == (m, 2, groups) and exps.dtype == torch.uint8
     assert torch.equal(out, M.gated_linear(x.cuda(), w.cuda(), b.cuda(), "silu"))
-    vals = codes.cpu().float().double().reshape(m, 2, f)
+    vals = codes.cpu().float().double()[:, :, :f]
     held = torch.cat([FO.unpack8(vals[:, h], exps.cpu()[:, h], F32) for h in range(2)], dim=1)
     unit = torch.ldexp(torch.ones(exps.shape, dtype=torch.float64), exps.cpu().to(torch.int64) - 127)
     per = torch.cat([unit[:, h].repeat_interleave(32, dim=1)[:, :f] for h in range(2)], dim=1)
@@ -418,7 +420,7 @@ def test_gated_linear_outputs_end_where_they_should():
         X, W, B, D = x.cuda(), w.cuda(), b.cuda(), do.cuda()
         mark = 123.0
         bufs = {n: torch.full((s + 2 * 512,), mark, dtype=t, device="cuda") for n, s, t in
-                (("out", m * f, dtype), ("z", m * 2 * f, dtype), ("z_aux", m * 2 * f, torch.uint8), ("d_x", m * k, dtype), ("d_weight", 2 * f * k, dtype),
+                (("out", m * f, dtype), ("z", m * 2 * ((f + 31) // 32 * 32), dtype), ("z_aux", m * 2 * ((f + 31) // 32 * 32), torch.uint8), ("d_x", m * k, dtype), ("d_weight", 2 * f * k, dtype),
                  ("d_bias", 2 * f, dtype))}
         at = {n: t.data_ptr() + 512 * t.element_size() for n, t in bufs.items()}
         p = _capi.HstuGatedParams(struct_size=C.sizeof(_capi.HstuGatedParams), dtype=code, bias_dtype=code, act=0, keep=1, k=k, f=f, m=m, x_stride=k,
