@@ -440,6 +440,21 @@ at::Tensor activation_unpack8(const at::Tensor& codes, const at::Tensor& exponen
     return out;
 }
 
+// The plain ops have no backward: under autograd, with an input that asks for gradients, they refuse instead of losing them.
+template <typename Fn, Fn fn> struct NoGrad;
+template <typename R, typename... Args, R (*fn)(Args...)> struct NoGrad<R (*)(Args...), fn> {
+    static bool asks(const at::Tensor& t) { return t.defined() && t.requires_grad(); }
+    static bool asks(const c10::optional<at::Tensor>& t) { return t.has_value() && asks(*t); }
+    template <typename T> static bool asks(const T&) { return false; }
+    static R call(Args... args) {
+        TORCH_CHECK(!at::GradMode::is_enabled() || !(asks(args) || ...),
+                    "mxrec: this op has no backward: call it under torch.no_grad(), on detached tensors, or use layer_norm / gated_linear");
+        at::AutoDispatchBelowADInplaceOrView guard;
+        return fn(args...);
+    }
+};
+#define FFN_NO_GRAD(f) TORCH_FN((NoGrad<decltype(&f), &f>::call))
+
 TORCH_LIBRARY_FRAGMENT(mxrec, m) {
     m.def("layer_norm(Tensor x, Tensor? weight, Tensor? bias, float eps=1e-05) -> Tensor");
     m.def("layer_norm_forward(Tensor x, Tensor? weight, Tensor? bias, float eps=1e-05) -> Tensor[]");
@@ -467,6 +482,12 @@ TORCH_LIBRARY_IMPL(mxrec, CPU, m) { FFN_IMPLS(m) }
 TORCH_LIBRARY_IMPL(mxrec, AutogradCUDA, m) {
     m.impl("layer_norm", TORCH_FN(layer_norm_autograd));
     m.impl("gated_linear", TORCH_FN(gated_linear_autograd));
+    m.impl("layer_norm_forward", FFN_NO_GRAD(layer_norm_forward));
+    m.impl("layer_norm_backward", FFN_NO_GRAD(layer_norm_backward));
+    m.impl("gated_linear_forward", FFN_NO_GRAD(gated_linear_forward));
+    m.impl("gated_linear_backward", FFN_NO_GRAD(gated_linear_backward));
+    m.impl("activation_pack8", FFN_NO_GRAD(activation_pack8));
+    m.impl("activation_unpack8", FFN_NO_GRAD(activation_unpack8));
 }
 
 }  // namespace mxrec_ffn

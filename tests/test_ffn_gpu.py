@@ -674,6 +674,20 @@ def test_gated_linear_keeps_nan_and_infinity_where_they_are():
             assert torch.equal(out[:, cols], clean[:, cols]) and bool(torch.isnan(out[:, 3]).all())
 
 
+def test_plain_ops_refuse_to_lose_gradients():
+    x, w = torch.randn(8, 64, device="cuda", dtype=BF, requires_grad=True), torch.randn(64, 64, device="cuda", dtype=BF)
+    one = torch.ones(64, device="cuda", dtype=BF)
+    y, mean, rstd = M.layer_norm_forward(x.detach(), one, one, EPS)
+    out, *kept = M.gated_linear_forward(x.detach(), w)
+    for call in (lambda: M.layer_norm_forward(x, one, one, EPS), lambda: M.layer_norm_forward(x.detach(), one.clone().requires_grad_(True), None, EPS),
+                 lambda: M.layer_norm_backward(y, x, one, mean, rstd), lambda: M.gated_linear_forward(x, w),
+                 lambda: M.gated_linear_backward(out, x, w, *kept), lambda: M.activation_pack8(x)):
+        with pytest.raises(RuntimeError, match="no backward"):
+            call()
+        with torch.no_grad():
+            call()
+
+
 def test_one_tensor_in_two_places():
     """The same tensor as x and weight, and as upstream gradient and input: gradients add up, results are the ones of copies."""
     t = torch.randn(64, 64, generator=torch.Generator().manual_seed(3)).to(BF).cuda()
