@@ -190,21 +190,22 @@ struct Plan { int tile, splits, tiles_n, tiles_m; int64_t c_split; double us; };
 // Tiles and shares of the contraction: the cheapest by a model of the launch, in microseconds.  A workgroup takes a start and an
 // end (`fixed`) and `piece` for each piece of its share; workgroups come in rounds of what the chip holds at a time; shares
 // beyond one cost a second kernel that adds their fp32 sums.
-// Measured (bf16): a piece of a 256 x 256 tile 1.6, of a 128 x 128 tile 0.55 alone on its CU with four buffers, 0.65 with two,
-// and 1.0 with two workgroups on a CU.  fp32 products are four times 128 x 128 x 32 in 1.8.
+// Measured (bf16, a full chip): a piece of a 256 x 256 tile 1.7, of a 256 x 128 one 1.1, of a 128 x 128 one 0.6 alone on its CU with
+// four buffers, 0.65 with two and 1.15 with two workgroups on a CU.  fp32 products are bound by their matrix rate: 128 x 128 x 32 in 1.8.
 static Plan gemm_plan(int kind, int32_t dtype, int64_t M, int64_t N, int64_t C) {
     const bool f32 = dtype == HSTU_F32;
     const int64_t bk = 128 / elem_bytes(dtype), pieces = (C + bk - 1) / bk;
     Plan best = {};
     double least = 1e300;
-    for (int tile = TILE_256; tile <= TILE_128_DEEP; tile++) {
+    for (int tile = 0; tile < GEMM_TILES; tile++) {
         const int64_t tm = (M + gemm_tile_m(tile) - 1) / gemm_tile_m(tile), tn = (N + gemm_tile_n(tile, kind) - 1) / gemm_tile_n(tile, kind);
         for (int splits = 1; splits <= 64; splits *= 2) {
             if (splits > 1 && (kind == GEMM_GATED || pieces < 2 * splits)) break;
             const double wgs = (double)tm * tn * splits, share = (double)((pieces + splits - 1) / splits);
             const bool pairs = tile == TILE_128 && wgs > 256;
-            const double piece = tile == TILE_256 ? (f32 ? 7.0 : 1.6) : f32 ? (pairs ? 3.6 : 1.8) : pairs ? 1.0 : tile == TILE_128 ? 0.65 : 0.55;
-            const double fixed = tile == TILE_256 ? 6.0 : pairs ? 4.0 : 3.0;
+            const double piece16[GEMM_TILES] = {1.7, pairs ? 1.15 : 0.65, 0.6, 1.1}, piece32[GEMM_TILES] = {7.0, pairs ? 3.6 : 1.8, 1.8, 3.5};
+            const double fixed_us[GEMM_TILES] = {6.0, pairs ? 4.0 : 3.0, 3.0, 4.5};
+            const double piece = f32 ? piece32[tile] : piece16[tile], fixed = fixed_us[tile];
             const double rounds = (double)(int64_t)((wgs + (pairs ? 511 : 255)) / (pairs ? 512 : 256));
             double t = rounds * (fixed + share * piece);
             if (splits > 1) t += 4.0 + (double)splits * M * N * 8 / 4.5e6;

@@ -421,9 +421,9 @@ __global__ __launch_bounds__(S::NT) void hstu_gemm_kernel(const GemmArgs a) {
 // kinds of products, and the launchers (one translation unit per element type)
 enum GemmKind : int { GEMM_GATED = 0 /* KC x KC, gated epilogue */, GEMM_DX = 1 /* n side RC, m side KC */, GEMM_DW = 2 /* both RC */ };
 // 256 x 256 outputs by eight waves (one workgroup per CU); 128 x 128 by four, with two buffers (two workgroups per CU) or four (one,
-// whose copies run three pieces ahead)
-enum GemmTile : int { TILE_256 = 0, TILE_128 = 1, TILE_128_DEEP = 2 };
-constexpr int gemm_tile_m(int tile) { return tile == TILE_256 ? 256 : 128; }
+// whose copies run three pieces ahead); 256 rows m x 128 by eight with three buffers (one)
+enum GemmTile : int { TILE_256 = 0, TILE_128 = 1, TILE_128_DEEP = 2, TILE_256x128 = 3, GEMM_TILES = 4 };
+constexpr int gemm_tile_m(int tile) { return tile == TILE_256 || tile == TILE_256x128 ? 256 : 128; }
 constexpr int gemm_tile_n(int tile, int kind) { return (tile == TILE_256 ? 256 : 128) / (kind == GEMM_GATED ? 2 : 1); }
 hipError_t launch_gemm_bf16(const GemmArgs& a, int kind, int tile, hipStream_t st);
 hipError_t launch_gemm_f16(const GemmArgs& a, int kind, int tile, hipStream_t st);
@@ -439,8 +439,11 @@ template <typename T> hipError_t launch_gemm_t(const GemmArgs& a, int kind, int 
         } else if (tile == TILE_128) {                                                                                          \
             typedef GemmShape<T, NRC, MRC, 128, 128, 2, 2, 2, GATED> S;                                                         \
             hipLaunchKernelGGL((hstu_gemm_kernel<S>), grid, dim3(S::NT), 0, st, a);                                             \
-        } else {                                                                                                                \
+        } else if (tile == TILE_128_DEEP) {                                                                                     \
             typedef GemmShape<T, NRC, MRC, 128, 128, 2, 2, 4, GATED> S;                                                         \
+            hipLaunchKernelGGL((hstu_gemm_kernel<S>), grid, dim3(S::NT), 0, st, a);                                             \
+        } else {                                                                                                                \
+            typedef GemmShape<T, NRC, MRC, 128, 256, 2, 4, 3, GATED> S;                                                         \
             hipLaunchKernelGGL((hstu_gemm_kernel<S>), grid, dim3(S::NT), 0, st, a);                                             \
         }                                                                                                                       \
     } while (0)
