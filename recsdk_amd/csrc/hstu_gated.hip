@@ -191,7 +191,13 @@ struct Plan { int tile, splits, tiles_n, tiles_m; int64_t c_split; double us; };
 // end (`fixed`) and `piece` for each piece of its share; workgroups come in rounds of what the chip holds at a time; shares
 // beyond one cost a second kernel that adds their fp32 sums.
 // Measured (bf16, a full chip): a piece of a 256 x 256 tile 1.7, of a 256 x 128 one 1.1, of a 128 x 128 one 0.6 alone on its CU with
-// four buffers, 0.65 with two and 1.15 with two workgroups on a CU.  fp32 products are bound by their matrix rate: 128 x 128 x 32 in 1.8.
+// four buffers, 0.65 with two and 1.15 with two workgroups on a CU, of a 64 x 128 one 0.5 and 0.8.  fp32 products are bound by
+// their matrix rate: 128 x 128 x 32 in 1.8, 64 x 128 x 32 in 0.95.
+// Each tile has the sizes where it is the fastest (forward, us: 256 x 256, 128 x 128, 256 x 128, 64 x 128):
+//   2789 x 1008 x 2736 fp16 37 44 40 55;  16384 x 512 x 2048 bf16 90 91 87 109;  8000 x 128 x 512 bf16 10.4 7.5 7.5 9.0;
+//   256 x 1024 x 4096 bf16 26 12.4 16 9.2;  100 x 2000 x 4000 fp32 473 134 245 74
+// and 128 x 128 with four buffers where one workgroup per CU is left of a long contraction (d_x of 256 x 1024 x 4096 27.8, with two
+// buffers 28.2; d_weight of 4096 x 512 x 2048 51.0 and 56.9).
 static Plan gemm_plan(int kind, int32_t dtype, int64_t M, int64_t N, int64_t C) {
     const bool f32 = dtype == HSTU_F32;
     const int64_t bk = 128 / elem_bytes(dtype), pieces = (C + bk - 1) / bk;
@@ -202,9 +208,10 @@ static Plan gemm_plan(int kind, int32_t dtype, int64_t M, int64_t N, int64_t C) 
         for (int splits = 1; splits <= 64; splits *= 2) {
             if (splits > 1 && (kind == GEMM_GATED || pieces < 2 * splits)) break;
             const double wgs = (double)tm * tn * splits, share = (double)((pieces + splits - 1) / splits);
-            const bool pairs = tile == TILE_128 && wgs > 256;
-            const double piece16[GEMM_TILES] = {1.7, pairs ? 1.15 : 0.65, 0.6, 1.1}, piece32[GEMM_TILES] = {7.0, pairs ? 3.6 : 1.8, 1.8, 3.5};
-            const double fixed_us[GEMM_TILES] = {6.0, pairs ? 4.0 : 3.0, 3.0, 4.5};
+            const bool pairs = (tile == TILE_128 || tile == TILE_64x128) && wgs > 256;   // two workgroups on a CU
+            const double piece16[GEMM_TILES] = {1.7, pairs ? 1.15 : 0.65, 0.6, 1.1, pairs ? 0.8 : 0.5};
+            const double piece32[GEMM_TILES] = {7.0, pairs ? 3.6 : 1.8, 1.8, 3.5, pairs ? 1.8 : 0.95};
+            const double fixed_us[GEMM_TILES] = {6.0, pairs ? 4.0 : 3.0, 3.0, 4.5, pairs ? 3.0 : 2.5};
             const double piece = f32 ? piece32[tile] : piece16[tile], fixed = fixed_us[tile];
             const double rounds = (double)(int64_t)((wgs + (pairs ? 511 : 255)) / (pairs ? 512 : 256));
             double t = rounds * (fixed + share * piece);

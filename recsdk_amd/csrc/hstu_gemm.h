@@ -1,17 +1,25 @@
 // Matrix-core product of the gated projection and of its backward: out[m, n] = sum over c of M[m, c] * N[n, c].
 //
 // A workgroup owns BM x BN outputs and walks the contraction in pieces of 128 bytes (64 columns of 16 bits, 32 of fp32).
-// Both operands of a piece are copied global -> LDS by buffer loads that write LDS directly, into one of two buffers, while
-// the matrix cores work on the other; one barrier per piece.  The MFMA is issued with the n side as its A operand, so that
-// an accumulator register quad holds four consecutive n of one row m and a lane exchange of the two half-waves makes
-// 16-byte pieces of an output row.
+// Both operands of a piece are copied global -> LDS by buffer loads that write LDS directly, into a ring of two to four
+// buffers, while the matrix cores work on an older one; one barrier per piece.  The MFMA is issued with the n side as its A
+// operand, so that an accumulator register quad holds four consecutive n of one row m and a lane exchange of the two
+// half-waves makes 16-byte pieces of an output row.
 //
 // An operand lies in memory either with the contraction contiguous (KC: element (row, c) at row * ld + c) or with the rows
 // contiguous (RC: c * ld + row).  In LDS a KC operand is [rows][128 B], 16-byte chunk c of row r at position
 // c ^ ((r >> 1) & 7): a fragment is one 16-byte LDS read, and 16 rows of one chunk cover all 64 banks.  An RC operand is
-// [c][rows], read with the transposing LDS load (four c of one row per lane); chunk q of line c sits at q ^ 4 (c & 3), so that
-// the four lines such a load touches lie in different banks.  fp32 RC lines are read four bytes a lane (chunk q ^ 8 ((c >> 2) & 1)).
+// [c][rows], read with the transposing LDS load (four c of one row per lane), fp32 four bytes a lane; its chunks are turned
+// (line_swizzle) so that the lines that such a load touches lie in different banks.  Counters show no bank conflicts.
 // Out-of-range rows and c are never addressed: their loads carry an offset beyond the buffer and return zero.
+//
+// Bounded by the matrix cores once a product fills the chip: [8192, 8192] outputs over c = 8192 reach 1340 TFLOP/s in bf16, and
+// one large library product 1351.  Below that it is the start and the end of a tile that cost, 5 to 7 us per round of tiles: the
+// gated forward at 8192 x 1024 -> 2 * 4096, whose contraction is 16 pieces and whose end computes the activation and stores out
+// and the kept z, takes 126 us (1090 TFLOP/s), and its counters show the matrix cores busy for 45 % of it.
+// Tried at that size and slower: four waves of 128 x 128 (263 us against 140 at the time: no second wave covers the end of the
+// first), the next lines called into L2 early (143), accumulators that start at the bias (145), workgroups that go on to their
+// next tile and start its copies before their end (140, and registers spilled).
 #pragma once
 #include "hstu_ffn_common.h"
 
@@ -110,6 +118,13 @@ struct GemmShape {
     static_assert(BN % (8 * NW) == 0 && BM % (8 * NW) == 0, "whole copies per wave");
 };
 
+// what a chunk's place in line c of an RC operand is turned by: the four lines that a transposing load touches (the two, for
+// fp32) lie in different banks
+template <int ES, int LINE> __device__ __forceinline__ int line_swizzle(int c) {
+    if (ES == 4) return 8 * ((c >> 2) & 1);
+    return LINE >= 256 ? 4 * (c & 3) : 4 * ((c >> 1) & 1);
+}
+
 // offsets of one operand's copies: 1 KiB piece i of this wave
 template <typename S, bool RC, int ROWS, int CNT> struct Stager {
     unsigned voff[CNT];
@@ -132,7 +147,7 @@ template <typename S, bool RC, int ROWS, int CNT> struct Stager {
                 constexpr int LPL = LINE / 16;                  // lanes per line
                 static_assert(LPL <= 64, "a copy holds whole lines");
                 const int c = p * (1024 / LINE) + lane / LPL;
-                const int chunk = (lane % LPL) ^ (ES == 2 ? 4 * (c & 3) : 8 * ((c >> 2) & 1));
+                const int chunk = (lane % LPL) ^ line_swizzle<ES, LINE>(c);
                 c_of[i] = c;
                 voff[i] = chunk * EC < rows ? (unsigned)((int64_t)c * ld * ES + chunk * 16) : 0x80000000u;
             }
@@ -165,14 +180,14 @@ __device__ __forceinline__ typename GM<typename S::T>::frag read_frag(const char
         return *reinterpret_cast<const frag*>(t + (32 * blk + l32) * 128 + (((2 * s + g) ^ sw) << 4));
     } else if constexpr (S::ES == 2) {
         const int rho = (lane >> 2) & 3;
-        const int chunk = (4 * blk + 2 * (l32 >> 4) + ((lane & 3) >> 1)) ^ (4 * rho);
+        const int chunk = (4 * blk + 2 * (l32 >> 4) + ((lane & 3) >> 1)) ^ line_swizzle<2, ROWS * 2>(rho);
         const char* at = t + (16 * s + 8 * g + rho) * (ROWS * 2) + (chunk << 4) + 8 * (lane & 1);
         const gm_s16x4 a = read_tr(at);
         const gm_s16x4 b = read_tr(at + 4 * (ROWS * 2));
         const gm_s16x8 v = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
         return __builtin_bit_cast(frag, v);
     } else {
-        const int chunk = (8 * blk + (l32 >> 2)) ^ (8 * g);
+        const int chunk = (8 * blk + (l32 >> 2)) ^ line_swizzle<4, ROWS * 4>(4 * g);
         const char* at = t + (8 * s + 4 * g) * (ROWS * 4) + (chunk << 4) + 4 * (l32 & 3);
         frag v;
 #pragma unroll
@@ -421,9 +436,10 @@ __global__ __launch_bounds__(S::NT) void hstu_gemm_kernel(const GemmArgs a) {
 // kinds of products, and the launchers (one translation unit per element type)
 enum GemmKind : int { GEMM_GATED = 0 /* KC x KC, gated epilogue */, GEMM_DX = 1 /* n side RC, m side KC */, GEMM_DW = 2 /* both RC */ };
 // 256 x 256 outputs by eight waves (one workgroup per CU); 128 x 128 by four, with two buffers (two workgroups per CU) or four (one,
-// whose copies run three pieces ahead); 256 rows m x 128 by eight with three buffers (one)
-enum GemmTile : int { TILE_256 = 0, TILE_128 = 1, TILE_128_DEEP = 2, TILE_256x128 = 3, GEMM_TILES = 4 };
-constexpr int gemm_tile_m(int tile) { return tile == TILE_256 || tile == TILE_256x128 ? 256 : 128; }
+// whose copies run three pieces ahead); 256 rows m x 128 by eight with three buffers (one); 64 x 128 by four with
+// three (two), for products too small for the others
+enum GemmTile : int { TILE_256 = 0, TILE_128 = 1, TILE_128_DEEP = 2, TILE_256x128 = 3, TILE_64x128 = 4, GEMM_TILES = 5 };
+constexpr int gemm_tile_m(int tile) { return tile == TILE_256 || tile == TILE_256x128 ? 256 : tile == TILE_64x128 ? 64 : 128; }
 constexpr int gemm_tile_n(int tile, int kind) { return (tile == TILE_256 ? 256 : 128) / (kind == GEMM_GATED ? 2 : 1); }
 hipError_t launch_gemm_bf16(const GemmArgs& a, int kind, int tile, hipStream_t st);
 hipError_t launch_gemm_f16(const GemmArgs& a, int kind, int tile, hipStream_t st);
@@ -442,8 +458,11 @@ template <typename T> hipError_t launch_gemm_t(const GemmArgs& a, int kind, int 
         } else if (tile == TILE_128_DEEP) {                                                                                     \
             typedef GemmShape<T, NRC, MRC, 128, 128, 2, 2, 4, GATED> S;                                                         \
             hipLaunchKernelGGL((hstu_gemm_kernel<S>), grid, dim3(S::NT), 0, st, a);                                             \
-        } else {                                                                                                                \
+        } else if (tile == TILE_256x128) {                                                                                      \
             typedef GemmShape<T, NRC, MRC, 128, 256, 2, 4, 3, GATED> S;                                                         \
+            hipLaunchKernelGGL((hstu_gemm_kernel<S>), grid, dim3(S::NT), 0, st, a);                                             \
+        } else {                                                                                                                \
+            typedef GemmShape<T, NRC, MRC, 128, 64, 2, 2, 3, GATED> S;                                                          \
             hipLaunchKernelGGL((hstu_gemm_kernel<S>), grid, dim3(S::NT), 0, st, a);                                             \
         }                                                                                                                       \
     } while (0)

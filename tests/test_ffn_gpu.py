@@ -292,7 +292,9 @@ def test_gated_linear_larger_and_reproducible(m, k, f, dtype, act):
                                                 (9000, 1100, 2200, BF, "silu", False), (33000, 520, 264, HF, "silu", True), (16384, 512, 2048, F32, "silu", False),
                                                 (70, 4096, 12000, BF, "silu", False), (24000, 16, 40, BF, "gelu", False),
                                                 (8000, 521, 100, BF, "silu", False), (1001, 520, 4000, HF, "silu", False), (8000, 520, 523, BF, "silu", True),
-                                                (4000, 1000, 520, HF, "gelu", False), (4001, 72, 520, BF, "silu", False), (12000, 520, 1000, HF, "silu", False)])
+                                                (4000, 1000, 520, HF, "gelu", False), (4001, 72, 520, BF, "silu", False), (12000, 520, 1000, HF, "silu", False),
+                                                (500, 264, 700, BF, "silu", False), (1000, 520, 2000, HF, "gelu", True), (300, 500, 1500, F32, "silu", False),
+                                                (129, 513, 2047, BF, "gelu", False)])
 def test_gated_linear_every_tile(m, k, f, dtype, act, c8):
     """Sizes at which the products run in each of their tiles, with and without shares of the contraction (64-bit oracle on the GPU)."""
     say("gated_linear tiles", m, k, f, dtype, act, c8)
