@@ -123,7 +123,8 @@ typedef struct hstu_gated_params {
 int hstu_hip_gated_linear_get_workspace_size(const hstu_gated_params* p, uint64_t* workspace_bytes);
 int hstu_hip_gated_linear(const hstu_gated_params* p, void* workspace, uint64_t workspace_bytes, void* stream);
 
-/* Backward:  dz_g = d_out * z_u * act'(z_g)     dz_u = d_out * act(z_g)     (rounded to dtype for the two products)
+/* Backward:  dz_g = d_out * z_u * act'(z_g)     dz_u = d_out * act(z_g)     (rounded to dtype for the two products,
+ *            so in HSTU_F16 within its range)
  *            d_x = dz W  [m, k]     d_weight = dz^T x  [2 f, k]     d_bias = column sums of the unrounded dz  [2 f]
  * Any of the three outputs may be NULL (not wanted). */
 typedef struct hstu_gated_bwd_params {

@@ -5,7 +5,8 @@ Importing the package loads the two shared libraries built by ``recsdk_amd._buil
 * ``lib/libhstu_hip.so``       C ABI (``include/hstu_hip.h``) + hand-written HIP kernels
 * ``lib/libmxrec_hstu_ops.so`` registers ``torch.ops.mxrec.hstu_jagged`` (``.equal`` / ``.delta``),
   ``hstu_paged``, ``hstu_dense`` with the reference's schemas, plus ``hstu_jagged_table_bias`` and
-  ``hstu_paged_fp8``
+  ``hstu_paged_fp8``, the layer steps, and the feed-forward half of a layer (``layer_norm``,
+  ``gated_linear``, ``activation_pack8``, ``activation_unpack8``)
 
 The loading convention is the reference's own: one ``torch.ops.load_library`` call
 (cust_op/rec_cust_ops/__init__.py:134-183).  There is no fallback implementation: if a library is

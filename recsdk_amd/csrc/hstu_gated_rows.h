@@ -5,6 +5,8 @@
 // turn, and a lane's 16-byte loads of W and x are MFMA fragments as they come (16 x 16 blocks, W as the A operand).  Rows of any
 // alignment are read in place; the last piece of a row goes by elements.  The waves' fp32 sums meet in LDS and are added in order.
 // Bounded by reading W: 16 FB columns a workgroup make f / 16 workgroups, and every wave has a whole piece per operand in flight.
+// One row, 1024 -> 4096: 3.3 us (16.8 MB of W; 5.1 TB/s, part of it out of the cache), with 32 columns a workgroup 6.2, with the next
+// piece under way 4.0.  48 rows: 7.1 to 7.7 us, in which each workgroup reads all of x.
 #pragma once
 #include "hstu_gemm.h"
 
