@@ -7,7 +7,8 @@
  * hstu_status with the message in hstu_hip_last_error().  Pointers need the alignment of their element type only, except
  * workspaces (16 bytes).  Outputs must not overlap inputs or each other.  A workspace needs no initialisation, belongs to one
  * call at a time and is free again when the call's work on the stream is done.  Sums over rows are formed in a fixed order:
- * results are reproducible.
+ * results are reproducible.  A call whose work would not fit one launch (more elements than the memory holds, unless rows repeat) is
+ * refused with HSTU_ERR_UNSUPPORTED.
  */
 #ifndef HSTU_FFN_H
 #define HSTU_FFN_H

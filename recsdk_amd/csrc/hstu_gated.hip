@@ -188,6 +188,8 @@ static hipError_t launch_gemm(int32_t dtype, const GemmArgs& a, int kind, int ti
     return launch_gemm_bf16(a, kind, tile, st);
 }
 
+// a launch holds less than 2^32 threads, a workgroup up to 512
+constexpr int64_t GEMM_MAX_TILES = 0x7fffff;
 struct Plan { int tile, splits, tiles_n, tiles_m; int64_t c_split; double us; };
 
 // Tiles and shares of the contraction: the cheapest by a model of the launch, in microseconds.  A workgroup takes a start and an
@@ -206,10 +208,11 @@ static Plan gemm_plan(int kind, int32_t dtype, int64_t M, int64_t N, int64_t C) 
     const int64_t bk = 128 / elem_bytes(dtype), pieces = (C + bk - 1) / bk;
     Plan best = {};
     double least = 1e300;
-    for (int tile = 0; tile < GEMM_TILES; tile++) {
+    for (int tile = 0; tile < GEMM_TILES; tile++) {   // (the first one also takes what would be too many tiles of the others)
         const int64_t tm = (M + gemm_tile_m(tile) - 1) / gemm_tile_m(tile), tn = (N + gemm_tile_n(tile, kind) - 1) / gemm_tile_n(tile, kind);
         for (int splits = 1; splits <= 64; splits *= 2) {
             if (splits > 1 && (kind == GEMM_GATED || pieces < 2 * splits)) break;
+            if (tm * tn * splits > GEMM_MAX_TILES && (tile != TILE_256 || splits > 1)) break;
             const double wgs = (double)tm * tn * splits, share = (double)((pieces + splits - 1) / splits);
             const bool pairs = (tile == TILE_128 || tile == TILE_64x128) && wgs > 256;   // two workgroups on a CU
             const double piece16[GEMM_TILES] = {1.7, pairs ? 1.15 : 0.65, 0.6, 1.1, pairs ? 0.8 : 0.5};
@@ -235,7 +238,7 @@ static Plan gemm_plan(int kind, int32_t dtype, int64_t M, int64_t N, int64_t C) 
 }
 
 static int gemm_too_large(const Plan& p) {
-    if ((int64_t)p.tiles_m * p.tiles_n * p.splits > 0x7fffffffLL) return fail(HSTU_ERR_UNSUPPORTED, "m * f too large for one launch");
+    if ((int64_t)p.tiles_m * p.tiles_n * p.splits > GEMM_MAX_TILES) return fail(HSTU_ERR_UNSUPPORTED, "m * f too large for one launch");
     return HSTU_OK;
 }
 
@@ -489,10 +492,8 @@ extern "C" int hstu_hip_gated_linear_backward(const hstu_gated_bwd_params* p, vo
         d.partial = p->d_bias ? reinterpret_cast<float*>(ws + l.sums) : nullptr;
         d.m = p->m; d.dout_stride = p->dout_stride; d.ld = l.ld; d.rows_wg = l.rows_wg;
         d.f = p->f; d.act = p->act; d.keep = p->keep; d.lanes = l.lanes; d.col_blocks = l.col_blocks;
-        const int64_t blocks = l.row_blocks * l.col_blocks;
-        if (blocks > 0x7fffffffLL) return fail(HSTU_ERR_UNSUPPORTED, "m * f too large for one launch");
         // without rows the workgroups write zero sums
-        const dim3 grid((unsigned)blocks);
+        const dim3 grid((unsigned)(l.row_blocks * l.col_blocks));
         if (p->dtype == HSTU_F32) hipLaunchKernelGGL(hstu_gated_dz_kernel<float>, grid, dim3(256), 0, st, d);
         else if (p->dtype == HSTU_F16) hipLaunchKernelGGL(hstu_gated_dz_kernel<_Float16>, grid, dim3(256), 0, st, d);
         else hipLaunchKernelGGL(hstu_gated_dz_kernel<__bf16>, grid, dim3(256), 0, st, d);

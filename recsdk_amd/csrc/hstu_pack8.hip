@@ -88,7 +88,7 @@ template <bool PACK> static int p8_run(const hstu_pack8_params* p, void* stream)
     if (p->rows == 0) return HSTU_OK;
     const int lanes = p8_lanes(p->cols), col_blocks = (p->cols + lanes * 8 - 1) / (lanes * 8);
     const int64_t per = (int64_t)(P8_NT / lanes) * P8_ROWS, blocks = (p->rows + per - 1) / per * col_blocks;
-    if (blocks > 0x7fffffffLL) return fail(HSTU_ERR_UNSUPPORTED, "rows * cols too large for one launch");
+    if (blocks > 0xffffff) return fail(HSTU_ERR_UNSUPPORTED, "rows * cols too large for one launch");
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     const dim3 grid((unsigned)blocks);
     if (p->dtype == HSTU_F32) hipLaunchKernelGGL((hstu_pack8_kernel<float, PACK>), grid, dim3(P8_NT), 0, st, *p, lanes, col_blocks);

@@ -239,3 +239,16 @@ def test_c_abi_pack8():
         assert fn(C.byref(p), None) == 0
     p = _fill(P, x_stride=511)
     assert L.hstu_hip_activation_unpack8(C.byref(p), None) == -1 and "at least cols" in _err()
+
+
+def test_c_abi_refuses_what_one_launch_does_not_hold():
+    """A launch holds less than 2^32 threads: the largest rows by the largest columns are refused before anything is launched."""
+    L = _capi.lib()
+    rows = 1 << 30
+    for fn in (L.hstu_hip_activation_pack8, L.hstu_hip_activation_unpack8):
+        p = _fill(_capi.HstuPack8Params, rows=rows, cols=65536, x_stride=65536)
+        assert fn(C.byref(p), None) == -2 and "too large for one launch" in _err()
+    p = _fill(_capi.HstuGatedParams, m=rows, k=512, x_stride=512, f=32768)
+    assert L.hstu_hip_gated_linear(C.byref(p), 0x10000, 1 << 62, None) == -2 and "too large for one launch" in _err()
+    p = _fill(_capi.HstuGatedBwdParams, m=rows, k=16384, x_stride=16384, f=32, dout_stride=32)
+    assert L.hstu_hip_gated_linear_backward(C.byref(p), 0x10000, 1 << 62, None) == -2 and "too large for one launch" in _err()
