@@ -103,20 +103,33 @@ template <typename T> __device__ __forceinline__ void store8_any(T* p, int n, co
 // ---- the gated product's activation ------------------------------------------------------------------------------------
 // silu(z) = z / (1 + e^-z); e^-z by the base-2 exponential instruction: the rounding of its argument costs |z| 2^-24 relative
 __device__ __forceinline__ float sigmoid_of(float z) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * z)); }
-__device__ __forceinline__ float act_of(float z, int act) {
-    if (act == HSTU_ACT_SILU) return z * sigmoid_of(z);
-    return 0.5f * z * erfcf(-0.70710678f * z);
+// N values at a time: one branch, and the exponentials and reciprocals of all of them under way together
+template <int N> __device__ __forceinline__ void act_of(const float* z, int act, float* a) {
+    if (act == HSTU_ACT_SILU) {
+#pragma unroll
+        for (int k = 0; k < N; k++) a[k] = z[k] * sigmoid_of(z[k]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; k++) a[k] = 0.5f * z[k] * erfcf(-0.70710678f * z[k]);
+    }
 }
 // act and its derivative
-__device__ __forceinline__ void act_and_grad(float z, int act, float& a, float& d) {
+template <int N> __device__ __forceinline__ void act_and_grad(const float* z, int act, float* a, float* d) {
     if (act == HSTU_ACT_SILU) {
-        const float s = sigmoid_of(z);
-        a = z * s;
-        d = __builtin_fmaf(a, 1.0f - s, s);   // s (1 + z (1 - s))
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+            const float s = sigmoid_of(z[k]);
+            a[k] = z[k] * s;
+            d[k] = __builtin_fmaf(a[k], 1.0f - s, s);   // s (1 + z (1 - s))
+        }
     } else {
-        const float phi = 0.5f * erfcf(-0.70710678f * z);
-        a = z * phi;
-        d = phi + z * 0.39894228f * __builtin_amdgcn_exp2f(-0.72134752f * z * z);
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+            const float phi = 0.5f * erfcf(-0.70710678f * z[k]);
+            a[k] = z[k] * phi;
+            d[k] = phi + z[k] * 0.39894228f * __builtin_amdgcn_exp2f(-0.72134752f * z[k] * z[k]);
+            __builtin_amdgcn_sched_barrier(0);   // (one erfc at a time: side by side they cost the row work its occupancy)
+        }
     }
 }
 

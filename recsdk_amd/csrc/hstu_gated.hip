@@ -82,13 +82,12 @@ __global__ __launch_bounds__(256) void hstu_gated_dz_kernel(const DzArgs a) {
                 join24(ug.q[0], lg.q, zg);
                 join24(uu.q[0], lu.q, zu);
             }
-            float dg[8], du[8];
+            float dg[8], du[8], act[8], grad[8];
+            act_and_grad<8>(zg, a.act, act, grad);
 #pragma unroll
             for (int k = 0; k < 8; k++) {
-                float act, grad;
-                act_and_grad(zg[k], a.act, act, grad);
-                dg[k] = d[k] * zu[k] * grad;
-                du[k] = d[k] * act;
+                dg[k] = d[k] * zu[k] * grad[k];
+                du[k] = d[k] * act[k];
                 sg[k] += dg[k];
                 su[k] += du[k];
             }

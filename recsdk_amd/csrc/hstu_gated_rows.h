@@ -144,7 +144,9 @@ __global__ __launch_bounds__(64 * ROWS_WAVES) void hstu_gated_rows_kernel(const 
     for (int v = threadIdx.x; v < a.m * 16 * FB; v += 64 * W) {
         const int m = v / (16 * FB), c = v % (16 * FB), f = f0 + c;
         const float zg = zs[0][m][c], zu = zs[1][m][c];
-        if (f < a.f) reinterpret_cast<T*>(a.out)[(int64_t)m * a.f + f] = from_float<T>(act_of(zg, a.act) * zu);
+        float act;
+        act_of<1>(&zg, a.act, &act);
+        if (f < a.f) reinterpret_cast<T*>(a.out)[(int64_t)m * a.f + f] = from_float<T>(act * zu);
         if (a.keep == HSTU_KEEP_FULL) {
             const int kept = HSTU_GATED_KEPT(a.f);   // (the grid covers the kept columns, and only those)
             const int64_t at = (int64_t)m * 2 * kept + f;

@@ -388,9 +388,7 @@ __global__ __launch_bounds__(S::NT) void hstu_gemm_kernel(const GemmArgs a) {
             for (int r = 0; r < 16; r++) {
                 zg[r] = acc[gb][j][r] + bg[r];
                 zu[r] = acc[NB / 2 + gb][j][r] + bu[r];
-                h[r] = act_of(zg[r], a.act) * zu[r];
             }
-            store_block<T>(reinterpret_cast<T*>(a.out) + m * a.N + n, h, g, left);
             // kept rows are padded to whole blocks; columns past f hold zero (no weight row, no bias)
             const int64_t kept = HSTU_GATED_KEPT((int64_t)a.N);
             const int whole = left > 0 ? 32 : 0;
@@ -428,6 +426,10 @@ __global__ __launch_bounds__(S::NT) void hstu_gemm_kernel(const GemmArgs a) {
                     if (g == 0 && left > 0) a.z_aux[((m * 2 + part) * kept + n) / HSTU_PACK8_GROUP] = (uint8_t)e;
                 }
             }
+            act_of<16>(zg, a.act, h);
+#pragma unroll
+            for (int r = 0; r < 16; r++) h[r] *= zu[r];
+            store_block<T>(reinterpret_cast<T*>(a.out) + m * a.N + n, h, g, left);
         }
         }
     }
