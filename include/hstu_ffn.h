@@ -97,7 +97,8 @@ int hstu_hip_activation_unpack8(const hstu_pack8_params* p, void* stream);
  * 16 bits of the fp32 value in z, the next 8 in z_aux (1 + 8 + 15 bits; rounded to 16 bits, z alone would put as large an error into
  * the gradients as the rounding of dz and of the gradients themselves).  What is kept has rows of 2 fp columns, fp = f rounded up to
  * a multiple of 32 (HSTU_GATED_KEPT(f)): the gate's f, zeros, the values' f, zeros; in 8 bits z_aux has an exponent for each 32 of
- * them, [m, 2, fp / 32].  m may be 0. */
+ * them, [m, 2, fp / 32].  In the 16-bit upper parts alone, blocks of 32 columns of the gate and of the values take turns, so that a
+ * block of both is a line of 128 bytes: [m, fp / 32, 2, 32].  m may be 0. */
 #define HSTU_GATED_MAX_K 16384
 #define HSTU_GATED_MAX_F 32768
 #define HSTU_GATED_KEPT(f) (((f) + 31) / 32 * 32)
@@ -118,7 +119,7 @@ typedef struct hstu_gated_params {
     const void* weight;    /* [2 f, k], contiguous */
     const void* bias;      /* [2 f], or NULL */
     void* out;             /* [m, f], contiguous */
-    void* z;               /* HSTU_KEEP_FULL: [m, 2, fp] fp32 or 16-bit upper parts; HSTU_KEEP_8BIT: codes [m, 2, fp] */
+    void* z;               /* HSTU_KEEP_FULL: fp32 [m, 2, fp], or 16-bit upper parts [m, fp / 32, 2, 32]; HSTU_KEEP_8BIT: codes [m, 2, fp] */
     uint8_t* z_aux;        /* HSTU_KEEP_FULL of 16-bit dtypes: lower parts [m, 2, fp]; HSTU_KEEP_8BIT: exponents */
 } hstu_gated_params;
 int hstu_hip_gated_linear_get_workspace_size(const hstu_gated_params* p, uint64_t* workspace_bytes);

@@ -75,9 +75,9 @@ __global__ __launch_bounds__(256) void hstu_gated_dz_kernel(const DzArgs a) {
                 load8_any(z, 8, zg);
                 load8_any(z + kept, 8, zu);
             } else {
-                const T* z = reinterpret_cast<const T*>(a.z) + r * 2 * kept + c;
+                const T* z = reinterpret_cast<const T*>(a.z) + r * 2 * kept + 2 * c - (c & 31);   // blocks of 32: the gate's, the values'
                 const uint8_t* low = a.z_aux + r * 2 * kept + c;
-                const Raw8<T> ug = load8_raw(z, 8), uu = load8_raw(z + kept, 8);
+                const Raw8<T> ug = load8_raw(z, 8), uu = load8_raw(z + 32, 8);
                 const Codes8 lg = codes8_raw(low, 8, 0), lu = codes8_raw(low + kept, 8, 0);
                 join24(ug.q[0], lg.q, zg);
                 join24(uu.q[0], lu.q, zu);

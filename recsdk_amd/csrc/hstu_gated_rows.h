@@ -155,8 +155,9 @@ __global__ __launch_bounds__(64 * ROWS_WAVES) void hstu_gated_rows_kernel(const 
                 reinterpret_cast<T*>(a.z)[at + kept] = zu;
             } else {
                 const unsigned bg = __builtin_bit_cast(unsigned, zg), bu = __builtin_bit_cast(unsigned, zu);
-                reinterpret_cast<uint16_t*>(a.z)[at] = (uint16_t)(bg >> 16);
-                reinterpret_cast<uint16_t*>(a.z)[at + kept] = (uint16_t)(bu >> 16);
+                uint16_t* up = reinterpret_cast<uint16_t*>(a.z) + at + f - (f & 31);   // blocks of 32: the gate's, the values'
+                up[0] = (uint16_t)(bg >> 16);
+                up[32] = (uint16_t)(bu >> 16);
                 a.z_aux[at] = (uint8_t)(bg >> 8);
                 a.z_aux[at + kept] = (uint8_t)(bu >> 8);
             }

@@ -103,10 +103,15 @@ __device__ __forceinline__ void swap_halves(unsigned& a, unsigned& b) {
 template <int N> struct gm_const { static constexpr int value = N; };
 
 // ---- the kernel -----------------------------------------------------------------------------------------------------------
-template <typename T_, bool NRC_, bool MRC_, int BN_, int BM_, int WN_, int WM_, int STAGES_, bool GATED_>
+// GATE: -1 for a plain product, gate_of(act, keep) for the gated projection.  The end of a gated tile is long unrolled code, an
+// instance for each of its activations and kept formats: with one for all of them, behind branches, the forward of 1024 x 512 -> 2048
+// bf16 took 9.1 us for 8.6, that of 16384 x 1024 -> 4096 with kept z 314 for 309.
+constexpr int gate_of(int act, int keep) { return act << 2 | keep; }
+template <typename T_, bool NRC_, bool MRC_, int BN_, int BM_, int WN_, int WM_, int STAGES_, int GATE_>
 struct GemmShape {
     typedef T_ T;
-    static constexpr bool NRC = NRC_, MRC = MRC_, GATED = GATED_;
+    static constexpr bool NRC = NRC_, MRC = MRC_, GATED = GATE_ >= 0;
+    static constexpr int ACT = GATE_ >> 2, KEEP = GATE_ & 3;      // of a gated one
     static constexpr int ES = sizeof(T), EC = 16 / ES;            // bytes of an element, elements of a 16-byte chunk
     static constexpr int BN = BN_, BM = BM_, BK = 128 / ES;
     static constexpr int WN = WN_, WM = WM_, NW = WN * WM, NT = 64 * NW;
@@ -206,6 +211,51 @@ template <typename T> __device__ __forceinline__ void store_pairs(T* row, const 
         swap_halves(a1, b1);
         const int n = 16 * h + 8 * g;
         if (n < n_left) store16<T>(row + n, (gm_u4){a0, a1, b0, b1}, n_left - n);
+    }
+}
+// The upper parts of a row's 32 kept gate columns and of the 32 value columns beside them: pieces change lanes between the rows of a
+// block, so that one store covers 8 whole lines of 128 bytes.  Whole lines go past the caches, which leaves those to the operands:
+// forward of 16384 x 1024 -> 4096 bf16 334 -> 303 us.  (32-byte pieces of 32 rows, as the lanes have them, 690 past the caches; the lower
+// parts and 8-bit codes in lines of their own, 64 bytes, no gain and dz 94 -> 100 and 36 -> 43.)
+__device__ __forceinline__ void swap_rows16(unsigned& a, unsigned& b) {   // lanes l (of a) and l - 16 (of b) where l & 16
+    const auto r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+    a = r[0];
+    b = r[1];
+}
+__device__ __forceinline__ void swap_rows8(unsigned& a, unsigned& b) {    // the same with 8
+    const int x = __builtin_amdgcn_update_dpp((int)a, (int)b, 0x128, 0xf, 0xc, false);   // rotated by 8 within 16, into the upper 8
+    b = (unsigned)__builtin_amdgcn_update_dpp((int)b, (int)a, 0x128, 0xf, 0x3, false);
+    a = (unsigned)x;
+}
+__device__ __forceinline__ void stream16(void* p, unsigned a, unsigned b, unsigned c, unsigned d) {
+    __builtin_nontemporal_store((gm_u4){a, b, c, d}, reinterpret_cast<gm_u4_any*>(p));
+}
+// `block` is where the block's row 0 starts, `ld` from a row to the next, `rows` how many there are
+template <typename T> __device__ __forceinline__ void store_kept_pairs(T* block, int64_t ld, unsigned (&w)[2][8], int lane, int rows) {
+    unsigned p[2][2][4];
+#pragma unroll
+    for (int q = 0; q < 2; q++) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            unsigned* v = w[q] + 4 * h;
+            swap_halves(v[0], v[2]);
+            swap_halves(v[1], v[3]);
+#pragma unroll
+            for (int i = 0; i < 4; i++) p[q][h][i] = v[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) swap_rows16(p[q][0][i], p[q][1][i]);
+    }
+#pragma unroll
+    for (int k = 0; k < 2; k++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) swap_rows8(p[0][k][i], p[1][k][i]);
+    const int at = 32 * ((lane >> 3) & 1) + 16 * ((lane >> 4) & 1) + 8 * (lane >> 5);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int r = 8 * i + (lane & 7);
+        const unsigned* v = p[i & 1][i >> 1];
+        if (r < rows) stream16(block + r * ld + at, v[0], v[1], v[2], v[3]);
     }
 }
 // as quads of bytes
@@ -389,26 +439,27 @@ __global__ __launch_bounds__(S::NT) void hstu_gemm_kernel(const GemmArgs a) {
                 zg[r] = acc[gb][j][r] + bg[r];
                 zu[r] = acc[NB / 2 + gb][j][r] + bu[r];
             }
-            // kept rows are padded to whole blocks; columns past f hold zero (no weight row, no bias)
+            // kept rows hold whole blocks; columns past f hold zero (no weight row, no bias)
             const int64_t kept = HSTU_GATED_KEPT((int64_t)a.N);
             const int whole = left > 0 ? 32 : 0;
-            if (a.keep == HSTU_KEEP_FULL) {
+            if constexpr (S::KEEP == HSTU_KEEP_FULL && S::ES == 4) {
+#pragma unroll
+                for (int part = 0; part < 2; part++) store_block<T>(reinterpret_cast<T*>(a.z) + (m * 2 + part) * kept + n, part ? zu : zg, g, whole);
+            } else if constexpr (S::KEEP == HSTU_KEEP_FULL) {
+                unsigned up[2][8];
 #pragma unroll
                 for (int part = 0; part < 2; part++) {
                     const float* v = part ? zu : zg;
-                    const int64_t at = (m * 2 + part) * kept + n;
-                    if constexpr (S::ES == 4) store_block<T>(reinterpret_cast<T*>(a.z) + at, v, g, whole);
-                    else {
-                        unsigned up[8], low[4];
+                    unsigned low[4];
 #pragma unroll
-                        for (int i = 0; i < 8; i++) up[i] = upper_pair(v[2 * i], v[2 * i + 1]);
+                    for (int i = 0; i < 8; i++) up[part][i] = upper_pair(v[2 * i], v[2 * i + 1]);
 #pragma unroll
-                        for (int i = 0; i < 4; i++) low[i] = lower_quad(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-                        store_pairs(reinterpret_cast<T*>(a.z) + at, up, g, whole);
-                        store_quads(a.z_aux + at, low, g, whole);
-                    }
+                    for (int i = 0; i < 4; i++) low[i] = lower_quad(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                    store_quads(a.z_aux + (m * 2 + part) * kept + n, low, g, whole);
                 }
-            } else if (a.keep == HSTU_KEEP_8BIT) {
+                const int64_t b0 = m - l32;   // row 0 of the block
+                store_kept_pairs(reinterpret_cast<T*>(a.z) + b0 * 2 * kept + 2 * n, 2 * kept, up, lane, n < a.N ? (int)min(a.M - b0, (int64_t)32) : 0);
+            } else if constexpr (S::KEEP == HSTU_KEEP_8BIT) {
                 // the 32 columns of a row lie in the 16 registers of two lanes
 #pragma unroll
                 for (int part = 0; part < 2; part++) {
@@ -426,7 +477,7 @@ __global__ __launch_bounds__(S::NT) void hstu_gemm_kernel(const GemmArgs a) {
                     if (g == 0 && left > 0) a.z_aux[((m * 2 + part) * kept + n) / HSTU_PACK8_GROUP] = (uint8_t)e;
                 }
             }
-            act_of<16>(zg, a.act, h);
+            act_of<16>(zg, S::ACT, h);
 #pragma unroll
             for (int r = 0; r < 16; r++) h[r] *= zu[r];
             store_block<T>(reinterpret_cast<T*>(a.out) + m * a.N + n, h, g, left);
@@ -447,31 +498,31 @@ hipError_t launch_gemm_bf16(const GemmArgs& a, int kind, int tile, hipStream_t s
 hipError_t launch_gemm_f16(const GemmArgs& a, int kind, int tile, hipStream_t st);
 hipError_t launch_gemm_f32(const GemmArgs& a, int kind, int tile, hipStream_t st);
 
-template <typename T> hipError_t launch_gemm_t(const GemmArgs& a, int kind, int tile, hipStream_t st) {
+template <typename T, bool NRC, bool MRC, int GATE> void launch_gemm_tile(const GemmArgs& a, int tile, hipStream_t st) {
     const dim3 grid((unsigned)((int64_t)a.tiles_n * a.tiles_m * a.splits));
-#define GM_GO(NRC, MRC, GATED)                                                                                                  \
-    do {                                                                                                                        \
-        if (tile == TILE_256) {                                                                                                 \
-            typedef GemmShape<T, NRC, MRC, 256, 256, 4, 2, 2, GATED> S;                                                            \
-            hipLaunchKernelGGL((hstu_gemm_kernel<S>), grid, dim3(S::NT), 0, st, a);                                             \
-        } else if (tile == TILE_128) {                                                                                          \
-            typedef GemmShape<T, NRC, MRC, 128, 128, 2, 2, 2, GATED> S;                                                         \
-            hipLaunchKernelGGL((hstu_gemm_kernel<S>), grid, dim3(S::NT), 0, st, a);                                             \
-        } else if (tile == TILE_128_DEEP) {                                                                                     \
-            typedef GemmShape<T, NRC, MRC, 128, 128, 2, 2, 4, GATED> S;                                                         \
-            hipLaunchKernelGGL((hstu_gemm_kernel<S>), grid, dim3(S::NT), 0, st, a);                                             \
-        } else if (tile == TILE_256x128) {                                                                                      \
-            typedef GemmShape<T, NRC, MRC, 128, 256, 2, 4, 3, GATED> S;                                                         \
-            hipLaunchKernelGGL((hstu_gemm_kernel<S>), grid, dim3(S::NT), 0, st, a);                                             \
-        } else {                                                                                                                \
-            typedef GemmShape<T, NRC, MRC, 128, 64, 2, 2, 3, GATED> S;                                                          \
-            hipLaunchKernelGGL((hstu_gemm_kernel<S>), grid, dim3(S::NT), 0, st, a);                                             \
-        }                                                                                                                       \
-    } while (0)
-    if (kind == GEMM_GATED) GM_GO(false, false, true);
-    else if (kind == GEMM_DX) GM_GO(true, false, false);
-    else GM_GO(true, true, false);
-#undef GM_GO
+    auto go = [&](auto shape) {
+        typedef decltype(shape) S;
+        hipLaunchKernelGGL((hstu_gemm_kernel<S>), grid, dim3(S::NT), 0, st, a);
+    };
+    if (tile == TILE_256) go(GemmShape<T, NRC, MRC, 256, 256, 4, 2, 2, GATE>());
+    else if (tile == TILE_128) go(GemmShape<T, NRC, MRC, 128, 128, 2, 2, 2, GATE>());
+    else if (tile == TILE_128_DEEP) go(GemmShape<T, NRC, MRC, 128, 128, 2, 2, 4, GATE>());
+    else if (tile == TILE_256x128) go(GemmShape<T, NRC, MRC, 128, 256, 2, 4, 3, GATE>());
+    else go(GemmShape<T, NRC, MRC, 128, 64, 2, 2, 3, GATE>());
+}
+template <typename T> hipError_t launch_gemm_t(const GemmArgs& a, int kind, int tile, hipStream_t st) {
+    if (kind == GEMM_DX) launch_gemm_tile<T, true, false, -1>(a, tile, st);
+    else if (kind == GEMM_DW) launch_gemm_tile<T, true, true, -1>(a, tile, st);
+    else {
+        auto gated = [&](auto act) {
+            constexpr int ACT = decltype(act)::value;
+            if (a.keep == HSTU_KEEP_NONE) launch_gemm_tile<T, false, false, gate_of(ACT, HSTU_KEEP_NONE)>(a, tile, st);
+            else if (sizeof(T) == 4 || a.keep == HSTU_KEEP_FULL) launch_gemm_tile<T, false, false, gate_of(ACT, HSTU_KEEP_FULL)>(a, tile, st);
+            else if constexpr (sizeof(T) == 2) launch_gemm_tile<T, false, false, gate_of(ACT, HSTU_KEEP_8BIT)>(a, tile, st);
+        };
+        if (a.act == HSTU_ACT_SILU) gated(gm_const<HSTU_ACT_SILU>());
+        else gated(gm_const<HSTU_ACT_GELU>());
+    }
     return hipGetLastError();
 }
 

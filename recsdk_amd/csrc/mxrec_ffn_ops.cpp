@@ -250,9 +250,14 @@ static std::vector<int64_t> with_last(const at::Tensor& x, int64_t last) {
     return s;
 }
 
-// what the first plane of a kept z is typed as
-static at::ScalarType kept_type(const at::Tensor& x, bool checkpoint8) {
-    return checkpoint8 ? at::kFloat8_e4m3fn : x.scalar_type() == at::kFloat ? at::kFloat : at::kBFloat16;
+// type and shape of a kept z for rows like x, and the shape of what is kept beside it (empty: nothing).  In the upper parts of the 24-bit
+// z the gate's and the values' blocks of 32 columns take turns.
+struct Kept { at::ScalarType type; std::vector<int64_t> z, aux; };
+static Kept kept_like(const at::Tensor& x, int64_t f, bool checkpoint8) {
+    const int64_t m = row_count(x), fp = HSTU_GATED_KEPT(f);
+    if (checkpoint8) return {at::kFloat8_e4m3fn, {m, 2, fp}, {m, 2, fp / HSTU_PACK8_GROUP}};
+    if (x.scalar_type() == at::kFloat) return {at::kFloat, {m, 2, fp}, {}};
+    return {at::kBFloat16, {m, fp / 32, 2, 32}, {m, 2, fp}};
 }
 
 // {out}, {out, z} (fp32), {out, upper parts of z, lower parts} (16-bit types: z in 24 bits) or {out, codes, exponents}
@@ -261,11 +266,13 @@ static std::vector<at::Tensor> gl_forward(const at::Tensor& x, const at::Tensor&
     check_devices(GL, {&x, &weight, &bias});
     Launch launch(x);
     const at::Tensor xr = rows_of(x), w = weight.contiguous(), b = bias.defined() ? bias.contiguous() : bias;
-    const int64_t m = row_count(x), f = weight.size(0) / 2, kept = HSTU_GATED_KEPT(f);
+    const int64_t m = row_count(x), f = weight.size(0) / 2;
     std::vector<at::Tensor> outs{at::empty(with_last(x, f), x.options().memory_format(at::MemoryFormat::Contiguous))};
-    if (keep != HSTU_KEEP_NONE) outs.push_back(at::empty({m, 2, kept}, x.options().dtype(kept_type(x, keep == HSTU_KEEP_8BIT))));
-    if (keep == HSTU_KEEP_8BIT) outs.push_back(at::empty({m, 2, kept / HSTU_PACK8_GROUP}, x.options().dtype(at::kByte)));
-    else if (keep == HSTU_KEEP_FULL && x.scalar_type() != at::kFloat) outs.push_back(at::empty({m, 2, kept}, x.options().dtype(at::kByte)));
+    if (keep != HSTU_KEEP_NONE) {
+        const Kept k = kept_like(x, f, keep == HSTU_KEEP_8BIT);
+        outs.push_back(at::empty(k.z, x.options().dtype(k.type)));
+        if (!k.aux.empty()) outs.push_back(at::empty(k.aux, x.options().dtype(at::kByte)));
+    }
     hstu_gated_params p;
     std::memset(&p, 0, sizeof(p));
     p.struct_size = sizeof(p);
@@ -378,14 +385,14 @@ std::vector<at::Tensor> gated_linear_backward(const at::Tensor& d_out, const at:
     const at::Tensor aux = value(z_aux);
     const bool c8 = z.scalar_type() == at::kFloat8_e4m3fn;
     gl_check(x, weight, at::Tensor(), c8);
-    const int64_t m = row_count(x), f = weight.size(0) / 2, kept = HSTU_GATED_KEPT(f);
+    const int64_t f = weight.size(0) / 2;
+    const Kept k = kept_like(x, f, c8);
     TORCH_CHECK(d_out.scalar_type() == x.scalar_type() && d_out.sizes().vec() == with_last(x, f), GL, ": d_out must have the dtype of x and the shape of out");
-    TORCH_CHECK(z.numel() == m * 2 * kept && z.scalar_type() == kept_type(x, c8), GL, ": z must be what gated_linear_forward kept: [", m, ", 2, ", kept,
-                "], float32 for float32 rows, bfloat16 upper parts or float8_e4m3fn codes otherwise");
-    const int64_t want = c8 ? m * 2 * kept / HSTU_PACK8_GROUP : x.scalar_type() == at::kFloat ? 0 : m * 2 * kept;
-    TORCH_CHECK(want == 0 || (aux.defined() && aux.scalar_type() == at::kByte && aux.numel() == want), GL,
-                ": z_aux must be what gated_linear_forward kept beside z: uint8, ", want, " values");
-    return gl_backward(d_out, x, weight, z, want ? aux : at::Tensor(), act_code(activation), at::kFloat, true, true, true);
+    TORCH_CHECK(z.scalar_type() == k.type && z.sizes().vec() == k.z, GL, ": z must be what gated_linear_forward kept: ", k.type, " ", at::IntArrayRef(k.z));
+    const bool two = !k.aux.empty();
+    TORCH_CHECK(!two || (aux.defined() && aux.scalar_type() == at::kByte && aux.sizes().vec() == k.aux), GL,
+                ": z_aux must be what gated_linear_forward kept beside z: uint8 ", at::IntArrayRef(k.aux));
+    return gl_backward(d_out, x, weight, z, two ? aux : at::Tensor(), act_code(activation), at::kFloat, true, true, true);
 }
 
 // ---- 8-bit activations ---------------------------------------------------------------------------------------------------

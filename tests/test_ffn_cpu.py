@@ -125,14 +125,15 @@ def test_gated_linear_refusals():
                      (dict(), "no CPU implementation"), (dict(b_=None), "no CPU implementation"), (dict(b_=b.float()), "no CPU implementation")):
         with pytest.raises(RuntimeError, match=text):
             run(**kw)
-    z = torch.zeros(6, 2, 32, dtype=torch.bfloat16)                # what the forward keeps: rows of 2 x 32 columns for f = 10
+    z = torch.zeros(6, 1, 2, 32, dtype=torch.bfloat16)             # what the forward keeps: a block of 2 x 32 columns for f = 10
+    c = torch.zeros(6, 2, 32).to(torch.float8_e4m3fn)
     do = torch.zeros(6, 10, dtype=torch.bfloat16)
     for args, text in (((do[:5], x, w, z), "d_out must have"), ((do.float(), x, w, z), "d_out must have"), ((do, x, w, z[:5]), "z must be"),
                        ((do, x, w, z.float()), "z must be"), ((do, x, w, z), "z_aux must be"), ((do, x, w, z, torch.zeros(6, 2, 1, dtype=torch.uint8)), "z_aux must be"),
-                       ((do, x, w, z, torch.zeros(6, 2, 32)), "z_aux must be"), ((do, x, w, z.to(torch.float8_e4m3fn), torch.zeros(6, 1, dtype=torch.uint8)), "z_aux must be"),
+                       ((do, x, w, z, torch.zeros(6, 2, 32)), "z_aux must be"), ((do, x, w, c, torch.zeros(6, 1, dtype=torch.uint8)), "z_aux must be"),
                        ((do, x, w, z, torch.zeros(6, 2, 32, dtype=torch.uint8)), "no CPU implementation"),
-                       ((do, x, w, z.to(torch.float8_e4m3fn), torch.zeros(6, 2, 1, dtype=torch.uint8)), "no CPU implementation"),
-                       ((do.float(), x.float(), w.float(), z.float()), "no CPU implementation")):
+                       ((do, x, w, c, torch.zeros(6, 2, 1, dtype=torch.uint8)), "no CPU implementation"),
+                       ((do.float(), x.float(), w.float(), c.float()), "no CPU implementation")):
         with pytest.raises(RuntimeError, match=text):
             M.gated_linear_backward(*args)
 

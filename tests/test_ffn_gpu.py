@@ -230,6 +230,7 @@ def joined(f, z, aux=None):
     """z as the forward keeps it: fp32, or the upper 16 and the next 8 bits of the fp32 values (cut off: 2^-15 of the value)."""
     if z.dtype == F32:
         return z.cpu()[:, :, :f].reshape(z.shape[0], 2 * f)
+    z = z.transpose(1, 2).reshape(aux.shape)              # the gate's and the values' blocks of 32 columns take turns
     z, aux = z[:, :, :f].reshape(z.shape[0], 2 * f).contiguous(), aux[:, :, :f].reshape(z.shape[0], 2 * f)
     up, low = z.cpu().view(torch.int16).to(torch.int64) & 0xffff, aux.cpu().to(torch.int64)
     return (((up << 16) | (low << 8)) & 0xffffffff).to(torch.int64).where(up < 0x8000, (((up << 16) | (low << 8)) - (1 << 32))).to(torch.int32).view(F32)
@@ -251,8 +252,11 @@ def test_gated_linear_sizes(m, k, f, dtype):
         tz, to = gl_forward_tol(x, w, b, z0, act, dtype)
         out, z, *aux = M.gated_linear_forward(x.cuda(), w.cuda(), cu(b), act)
         within(out, out0, to, "out")
-        assert z.shape == (m, 2, (f + 31) // 32 * 32) and z.dtype == (F32 if dtype == F32 else BF) and len(aux) == (0 if dtype == F32 else 1)
-        assert not bool(z[:, :, f:].float().any())                     # zeros behind the columns
+        fp = (f + 31) // 32 * 32
+        assert z.shape == ((m, 2, fp) if dtype == F32 else (m, fp // 32, 2, 32)) and z.dtype == (F32 if dtype == F32 else BF)
+        assert [a.shape for a in aux] == ([] if dtype == F32 else [(m, 2, fp)])
+        rows = z if dtype == F32 else z.transpose(1, 2).reshape(m, 2, fp)
+        assert not bool(rows[:, :, f:].float().any()) and not any(bool(a[:, :, f:].any()) for a in aux)   # zeros behind the columns
         # the backward for the z that the forward kept
         zk = joined(f, z, *aux)
         within(zk, z0, tz + (U[F32] + CUT[dtype]) * z0.abs() + TINY[F32], "z")
