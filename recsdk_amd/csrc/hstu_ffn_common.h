@@ -74,7 +74,7 @@ template <typename T> __device__ __forceinline__ void to_floats(const Raw8<T>& r
     for (int k = 0; k < 8; k++) v[k] = to_float(t[k]);
 }
 template <typename T> __device__ __forceinline__ void load8_any(const T* p, int n, float* v) { to_floats(load8_raw(p, n), v); }
-template <typename T> __device__ __forceinline__ void store8_any(T* p, int n, const float* v) {
+template <bool STREAM = true, typename T> __device__ __forceinline__ void store8_any(T* p, int n, const float* v) {
     T t[8];
 #pragma unroll
     for (int k = 0; k < 8; k++) t[k] = from_float<T>(v[k]);
@@ -82,7 +82,10 @@ template <typename T> __device__ __forceinline__ void store8_any(T* p, int n, co
     __builtin_memcpy(&r, t, sizeof(r));
     if (n >= 8) {
 #pragma unroll
-        for (int q = 0; q < (int)(8 * sizeof(T) / 16); q++) __builtin_nontemporal_store(r.q[q], reinterpret_cast<ffn_u4_any*>(p) + q);
+        for (int q = 0; q < (int)(8 * sizeof(T) / 16); q++) {
+            if (STREAM) __builtin_nontemporal_store(r.q[q], reinterpret_cast<ffn_u4_any*>(p) + q);
+            else *(reinterpret_cast<ffn_u4_any*>(p) + q) = r.q[q];
+        }
         return;
     }
     if (n <= 0) return;

@@ -28,7 +28,7 @@ __global__ __launch_bounds__(256) void hstu_pad_rows_kernel(const PadArgs a) {
         for (int c = lane * 8; c < a.ld; c += 512) {
             float v[8];
             load8_any(src + c, a.cols - c, v);
-            store8_any(dst + c, (int)(a.ld - c), v);
+            store8_any<false>(dst + c, (int)(a.ld - c), v);   // (read again by the next launch)
         }
     }
 }
@@ -93,8 +93,8 @@ __global__ __launch_bounds__(256) void hstu_gated_dz_kernel(const DzArgs a) {
             }
             if (a.dz) {
                 T* dz = reinterpret_cast<T*>(a.dz) + r * a.ld + c;
-                store8_any(dz, n, dg);
-                store8_any(dz + a.f, n, du);
+                store8_any<false>(dz, n, dg);
+                store8_any<false>(dz + a.f, n, du);
                 if (n <= 8)
                     for (int64_t k = 2 * (int64_t)a.f; k < a.ld; k++) reinterpret_cast<T*>(a.dz)[r * a.ld + k] = from_float<T>(0.f);
             }
