@@ -195,7 +195,7 @@ struct Plan { int tile, splits, tiles_n, tiles_m; int64_t c_split; double us; };
 // end (`fixed`) and `piece` for each piece of its share; workgroups come in rounds of what the chip holds at a time; shares
 // beyond one cost a second kernel that adds their fp32 sums.
 // Measured (bf16, a full chip): a piece of a 256 x 256 tile 1.7, of a 256 x 128 one 1.1, of a 128 x 128 one 0.6 alone on its CU with
-// four buffers, 0.65 with two and 1.15 with two workgroups on a CU, of a 64 x 128 one 0.5 and 0.8.  fp32 products are bound by
+// four buffers, 0.65 with two and 1.15 with two workgroups on a CU, of a 64 x 128 one 0.42 and 0.8.  fp32 products are bound by
 // their matrix rate: 128 x 128 x 32 in 1.8, 64 x 128 x 32 in 0.95.
 // Each tile has the sizes where it is the fastest (forward, us: 256 x 256, 128 x 128, 256 x 128, 64 x 128):
 //   2789 x 1008 x 2736 fp16 37 44 40 55;  16384 x 512 x 2048 bf16 90 91 87 109;  8000 x 128 x 512 bf16 10.4 7.5 7.5 9.0;
@@ -214,7 +214,7 @@ static Plan gemm_plan(int kind, int32_t dtype, int64_t M, int64_t N, int64_t C) 
             if (tm * tn * splits > GEMM_MAX_TILES && (tile != TILE_256 || splits > 1)) break;
             const double wgs = (double)tm * tn * splits, share = (double)((pieces + splits - 1) / splits);
             const bool pairs = (tile == TILE_128 || tile == TILE_64x128) && wgs > 256;   // two workgroups on a CU
-            const double piece16[GEMM_TILES] = {1.7, pairs ? 1.15 : 0.65, 0.6, 1.1, pairs ? 0.8 : 0.5};
+            const double piece16[GEMM_TILES] = {1.7, pairs ? 1.15 : 0.65, 0.6, 1.1, pairs ? 0.8 : 0.42};
             const double piece32[GEMM_TILES] = {7.0, pairs ? 3.6 : 1.8, 1.8, 3.5, pairs ? 1.8 : 0.95};
             const double fixed_us[GEMM_TILES] = {6.0, pairs ? 4.0 : 3.0, 3.0, 4.5, pairs ? 3.0 : 2.5};
             const double piece = f32 ? piece32[tile] : piece16[tile], fixed = fixed_us[tile];
@@ -275,13 +275,23 @@ static int gated_check_sizes(int32_t dtype, int32_t act, int32_t keep, int64_t m
     return HSTU_OK;
 }
 
-// Few rows go to the kernel that reads W straight into fragments, as long as its workgroups' reading of x, f / 16 times, costs
-// less than tiles of 128 rows that are mostly empty.  Measured (bf16, k 1024): at f 4096, 4.3 us for one row and 8.1 for 64 against
-// 12.2 and 12.4 in tiles; at f 16384, 12.0 and 24.9 against 13.9 and 14.6, so that tiles take over at about 16 rows there.
+// Few rows go to the kernel that reads W straight into fragments where a model of both says that it is faster than tiles, most rows
+// of which are empty.  A workgroup of that kernel reads 32 rows of W and all of x, at a rate that two on a CU (up to 32 rows) or one have;
+// neither kernel reads W faster than memory gives it.  Measured (bf16, us, few rows / tiles):
+//   1024 -> 4096: one row 3.4 / 7.9, 48 4.7 / 8.1, 64 5.5 / 8.3;   -> 8192: 32 rows 5.7 / 7.9, 48 8.9 / 8.1, 64 10.8 / 8.3;
+//   512 -> 16384: one row 5.0 / 5.4, 32 7.7 / 5.8;   2048 -> 8192: 1 11.4 / 13.0, 48 16.1 / 13.5;   8192 -> 1024: 1 10.1 / 42, 64 20 / 43
+// (It takes 16 bytes of a row at a time, at 32-bit offsets within 16 rows.)
 static bool few_rows(const hstu_gated_params* p) {
-    if (p->m > ROWS_MAX_M) return false;
-    const double e = elem_bytes(p->dtype), w = 2.0 * p->f * p->k * e, x = (p->f / 16.0) * p->m * p->k * e;
-    return 2.2 + w / 7e6 + x / 9e6 <= gemm_plan(GEMM_GATED, p->dtype, p->m, p->f, p->k).us + 2.5;
+    const double e = elem_bytes(p->dtype);
+    if (p->m > ROWS_MAX_M || p->k < 16 / e || (p->m > 1 && p->x_stride > (1 << 20))) return false;
+    const int64_t mb = (p->m + 15) / 16, wgs = (p->f + 15) / 16;
+    const bool two = mb <= 2;
+    const double share = two && wgs > 256 ? 2 : 1, rounds = (double)((wgs + (two ? 511 : 255)) / (two ? 512 : 256));
+    const double bytes = (32.0 + 16.0 * mb) * p->k * e * share, fp32 = p->dtype == HSTU_F32 ? 1.9e-3 * share * mb * p->k : 0.0;
+    const double rows_us = 1.0 + rounds * (2.0 + bytes / (two ? 95e3 : 58e3) + fp32), least = 2.2 + 2.0 * p->f * p->k * e / 6.9e6;
+    const double pad = needs_pad(p->weight, p->k, p->k, p->dtype) ? 4.0 + 2.0 * p->f * p->k * e / 2e6 : 0.0;   // (1001 -> 6001: 24 MB, 16 us)
+    const double tiles_us = pad + (p->dtype == HSTU_F32 ? 1.15 : 0.87) * gemm_plan(GEMM_GATED, p->dtype, p->m, p->f, p->k).us;
+    return (rows_us > least ? rows_us : least) < (tiles_us > least ? tiles_us : least);
 }
 
 struct GatedLayout { uint64_t x, w, bytes; bool pad_x, pad_w; };

@@ -1,12 +1,14 @@
 // The gated projection for few rows (single tokens, the candidates of a request): act(x Wg^T + bg) * (x Wu^T + bu) with m <= 64.
 //
 // The weights are read once and there is nothing to share between workgroups but a few rows of x, so nothing goes through LDS on
-// the way in: a workgroup owns 16 FB columns f (their gate and their value rows), its eight waves take pieces of 128 bytes of k in
-// turn, and a lane's 16-byte loads of W and x are MFMA fragments as they come (16 x 16 blocks, W as the A operand).  Rows of any
-// alignment are read in place; the last piece of a row goes by elements.  The waves' fp32 sums meet in LDS and are added in order.
-// Bounded by reading W: 16 FB columns a workgroup make f / 16 workgroups, and every wave has a whole piece per operand in flight.
-// One row, 1024 -> 4096: 3.3 us (16.8 MB of W; 5.1 TB/s, part of it out of the cache), with 32 columns a workgroup 6.2, with the next
-// piece under way 4.0.  48 rows: 7.1 to 7.7 us, in which each workgroup reads all of x.
+// the way in: a workgroup owns 16 FB columns f (their gate and their value rows), its eight waves take pieces of 256 bytes of k in
+// turn.  Four neighbouring lanes load 64 bytes of a row, and a transpose over them makes MFMA fragments (16 x 16 blocks, W as the A
+// operand); loaded as fragments, 16 rows to 16 neighbouring lanes, a load brings 16 bytes a cycle into a CU for 64.  Rows of any
+// alignment are read in place; what the last piece of a row has of them is cut out of the row's last 16 bytes.  The waves' fp32 sums
+// meet in LDS and are added in order.
+// Bounded by reading W, for more rows by each workgroup's reading of all of x.  1024 -> 4096 bf16: one row 3.4 us (16.8 MB of W, part of
+// it out of the caches; 4.2 loaded as fragments), 48 rows 4.7 (7.0); 4096 -> 1024: one row 6.0 (10.3), 64 rows 11.5 (24).  32 columns a
+// workgroup are slower (6.2 for 4.3 at one row), and so is a second piece under way.
 #pragma once
 #include "hstu_gemm.h"
 
@@ -25,16 +27,20 @@ struct RowsArgs {
 constexpr int ROWS_MAX_M = 64;
 constexpr int ROWS_WAVES = 8;
 
-// 16 bytes of consecutive elements at any address, zero from element n on
-template <typename T> __device__ __forceinline__ typename GM<T>::frag load_frag(const T* p, int n) {
-    typedef typename GM<T>::frag frag;
-    constexpr int EC = 16 / sizeof(T);
-    if (n >= EC) return __builtin_bit_cast(frag, *reinterpret_cast<const gm_u4_any*>(p));
-    T e[EC];
+// the last n elements (all of them where n is larger, zeros where it is not positive) moved to the front, zeros behind
+template <typename T> __device__ __forceinline__ gm_u4 last_elements(gm_u4 v, int n) {
+    const int bytes = 16 - max(min(n * (int)sizeof(T), 16), 0);
+    if constexpr (sizeof(T) == 2) {
+        const bool half = bytes & 2;
 #pragma unroll
-    for (int i = 0; i < EC; i++) e[i] = i < n ? p[i] : from_float<T>(0.f);
-    frag v;
-    __builtin_memcpy(&v, e, 16);
+        for (int i = 0; i < 4; i++) {
+            const unsigned moved = __builtin_amdgcn_alignbit(i < 3 ? v[i < 3 ? i + 1 : 3] : 0u, v[i], 16);
+            v[i] = half ? moved : v[i];
+        }
+    }
+    if (bytes & 4) v = (gm_u4){v[1], v[2], v[3], 0u};
+    if (bytes & 8) v = (gm_u4){v[2], v[3], 0u, 0u};
+    if (bytes & 16) v = (gm_u4){0u, 0u, 0u, 0u};
     return v;
 }
 __device__ __forceinline__ gm_f32x4 mfma16(gm_bf16x8 a, gm_bf16x8 b, gm_f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
@@ -45,26 +51,60 @@ __device__ __forceinline__ gm_f32x4 mfma16(gm_f32x4 a, gm_f32x4 b, gm_f32x4 c) {
     return c;
 }
 
+// 4 x 4 transpose of 16-byte fragments over four neighbouring lanes: v[j] of lane s becomes v[s] of lane j
+template <int CTRL> __device__ __forceinline__ void exchange(unsigned& a, unsigned& b, bool upper) {
+    const unsigned from_b = (unsigned)__builtin_amdgcn_mov_dpp((int)b, CTRL, 0xf, 0xf, true), from_a = (unsigned)__builtin_amdgcn_mov_dpp((int)a, CTRL, 0xf, 0xf, true);
+    a = upper ? from_b : a;
+    b = upper ? b : from_a;
+}
+template <typename F> __device__ __forceinline__ void quad_transpose(F (&v)[4], int lane) {
+    gm_u4 u[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) u[i] = __builtin_bit_cast(gm_u4, v[i]);
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+        unsigned a = u[0][t], b = u[1][t], c = u[2][t], d = u[3][t];
+        exchange<0xB1>(a, b, lane & 1);   // quad_perm 1 0 3 2
+        exchange<0xB1>(c, d, lane & 1);
+        exchange<0x4E>(a, c, lane & 2);   // quad_perm 2 3 0 1
+        exchange<0x4E>(b, d, lane & 2);
+        u[0][t] = a;
+        u[1][t] = b;
+        u[2][t] = c;
+        u[3][t] = d;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] = __builtin_bit_cast(F, u[i]);
+}
+
 template <typename T, int MB, int FB>
 __global__ __launch_bounds__(64 * ROWS_WAVES) void hstu_gated_rows_kernel(const RowsArgs a) {
     typedef typename GM<T>::frag frag;
-    constexpr int EC = 16 / sizeof(T), PIECE = 8 * EC, W = ROWS_WAVES;
+    constexpr int ES = sizeof(T), EC = 16 / ES, PIECE = 16 * EC, W = ROWS_WAVES;
     constexpr int VALS = 2 * FB * MB * 256;            // fp32 sums of a wave
     __shared__ float red[W * VALS];
     __shared__ float zs[2][16 * MB][16 * FB + 1];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r16 = lane & 15, q = lane >> 4;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, q = lane >> 4;
     const int f0 = blockIdx.x * (16 * FB);
     const T* x = reinterpret_cast<const T*>(a.x);
     const T* wt = reinterpret_cast<const T*>(a.weight);
-    // rows behind the last one repeat it: their products are never stored
-    const T* wrow[2][FB];
-    const T* xrow[MB];
+    // Load i of a block: lane l takes chunk (l & 3) + 4 (l >> 4) of row 4 (l >> 2 & 3) + i.  After the transpose load j holds chunk
+    // j + 4 (l >> 4) of row l & 15, a fragment.  Rows behind the last one repeat it: their products are never stored
+    const int chunk = ((lane & 3) + 4 * q) * EC, fb = min(f0, a.f - 1);
+    const char* wb[2] = {reinterpret_cast<const char*>(wt + (int64_t)fb * a.k), reinterpret_cast<const char*>(wt + ((int64_t)a.f + fb) * a.k)};
+    const char* xb[MB];
+    unsigned wo[FB][4], xo[MB][4];   // bytes from there to the lane's row
 #pragma unroll
-    for (int h = 0; h < 2; h++)
+    for (int j = 0; j < MB; j++) xb[j] = reinterpret_cast<const char*>(x + (int64_t)(16 * j) * a.x_stride);
 #pragma unroll
-        for (int b = 0; b < FB; b++) wrow[h][b] = wt + ((int64_t)h * a.f + min(f0 + 16 * b + r16, a.f - 1)) * a.k + q * EC;
+    for (int i = 0; i < 4; i++) {
+        const int r = (lane & 12) + i;
 #pragma unroll
-    for (int j = 0; j < MB; j++) xrow[j] = x + (int64_t)min(16 * j + r16, a.m - 1) * a.x_stride + q * EC;
+        for (int b = 0; b < FB; b++) wo[b][i] = (unsigned)(min(f0 + 16 * b + r, a.f - 1) - fb) * (unsigned)a.k * ES;
+#pragma unroll
+        for (int j = 0; j < MB; j++) xo[j][i] = (unsigned)(min(16 * j + r, a.m - 1) - 16 * j) * (unsigned)a.x_stride * ES;
+    }
+    auto load = [](const char* at, unsigned off) __attribute__((always_inline)) { return *reinterpret_cast<const gm_u4_any*>(at + off); };
     gm_f32x4 acc[2][FB][MB];
 #pragma unroll
     for (int h = 0; h < 2; h++)
@@ -73,44 +113,51 @@ __global__ __launch_bounds__(64 * ROWS_WAVES) void hstu_gated_rows_kernel(const 
 #pragma unroll
             for (int j = 0; j < MB; j++) acc[h][b][j] = gm_f32x4{0.f, 0.f, 0.f, 0.f};
     // whole pieces without a branch between their loads; only a row's last piece may be shorter
-    struct Piece { frag w[2][2][FB], x[2][MB]; };
-    auto multiply = [&](const Piece& p) __attribute__((always_inline)) {
+    struct Piece { frag w[2][FB][4], x[MB][4]; };
+    auto multiply = [&](Piece& p) __attribute__((always_inline)) {
 #pragma unroll
-        for (int s = 0; s < 2; s++)
+        for (int j = 0; j < MB; j++) quad_transpose(p.x[j], lane);
 #pragma unroll
-            for (int h = 0; h < 2; h++)
+        for (int h = 0; h < 2; h++)
 #pragma unroll
-                for (int b = 0; b < FB; b++)
+            for (int b = 0; b < FB; b++) {
+                quad_transpose(p.w[h][b], lane);
 #pragma unroll
-                    for (int j = 0; j < MB; j++) acc[h][b][j] = mfma16(p.w[s][h][b], p.x[s][j], acc[h][b][j]);
+                for (int s = 0; s < 4; s++)
+#pragma unroll
+                    for (int j = 0; j < MB; j++) acc[h][b][j] = mfma16(p.w[h][b][s], p.x[j][s], acc[h][b][j]);
+            }
     };
     int k0 = w * PIECE;
-#pragma unroll 2
     for (; k0 + PIECE <= a.k; k0 += W * PIECE) {
+        const unsigned at = (unsigned)(k0 + chunk) * ES;
         Piece p;
 #pragma unroll
-        for (int s = 0; s < 2; s++) {
-            const int at = k0 + 4 * EC * s;
+        for (int j = 0; j < MB; j++)
 #pragma unroll
-            for (int h = 0; h < 2; h++)
+            for (int i = 0; i < 4; i++) p.x[j][i] = __builtin_bit_cast(frag, load(xb[j], xo[j][i] + at));
 #pragma unroll
-                for (int b = 0; b < FB; b++) p.w[s][h][b] = __builtin_bit_cast(frag, *reinterpret_cast<const gm_u4_any*>(wrow[h][b] + at));
+        for (int h = 0; h < 2; h++)
 #pragma unroll
-            for (int j = 0; j < MB; j++) p.x[s][j] = __builtin_bit_cast(frag, *reinterpret_cast<const gm_u4_any*>(xrow[j] + at));
-        }
+            for (int b = 0; b < FB; b++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) p.w[h][b][i] = __builtin_bit_cast(frag, load(wb[h], wo[b][i] + at));
+        __builtin_amdgcn_sched_barrier(0);
         multiply(p);
     }
     if (k0 < a.k) {
+        // a chunk that the row ends in is cut out of the row's last 16 bytes
+        const int n = a.k - k0 - chunk;
+        const unsigned at = (unsigned)(n >= EC ? k0 + chunk : a.k - EC) * ES;
         Piece p;
 #pragma unroll
-        for (int s = 0; s < 2; s++) {
-            const int at = k0 + 4 * EC * s, n = a.k - (at + q * EC), o = n > 0 ? at : 0;
+        for (int i = 0; i < 4; i++) {
 #pragma unroll
             for (int h = 0; h < 2; h++)
 #pragma unroll
-                for (int b = 0; b < FB; b++) p.w[s][h][b] = load_frag(wrow[h][b] + o, n);
+                for (int b = 0; b < FB; b++) p.w[h][b][i] = __builtin_bit_cast(frag, last_elements<T>(load(wb[h], wo[b][i] + at), n));
 #pragma unroll
-            for (int j = 0; j < MB; j++) p.x[s][j] = load_frag(xrow[j] + o, n);
+            for (int j = 0; j < MB; j++) p.x[j][i] = __builtin_bit_cast(frag, last_elements<T>(load(xb[j], xo[j][i] + at), n));
         }
         multiply(p);
     }

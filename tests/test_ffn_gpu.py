@@ -456,6 +456,20 @@ def test_gated_linear_outputs_end_where_they_should():
             assert torch.equal(g.flatten(), bufs[nm][512:-512]), nm
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("k", [1, 3, 8, 100, 133])
+def test_gated_linear_rows_far_apart(dtype, k):
+    """Few rows, 2^20 elements apart and a little more (which changes the kernel), against the 64-bit oracle."""
+    say("rows far apart", dtype, k)
+    x, w, b, _ = gl_case(5, k, 70, dtype, True, 77)
+    want, z = FO.gated_linear(x, w, b, "silu")
+    _, tol = gl_forward_tol(x, w, b, z, "silu", dtype)
+    for stride in (1 << 20, (1 << 20) + 1, (1 << 20) + 8):
+        far = torch.zeros(5 * stride, dtype=dtype, device="cuda").as_strided((5, k), (stride, 1))
+        far.copy_(x)
+        within(M.gated_linear(far, w.cuda(), b.cuda()), want, tol, "out")
+
+
 def test_gated_linear_gradient_against_differences():
     """Central differences of sum(out * d_out) in fp32, in a direction of each leaf."""
     x, w, b, do = gl_case(20, 48, 40, F32, True, 41)
