@@ -6,8 +6,8 @@
 //   backward  a = dy w, dx = rstd (a - (sum a + x_hat sum a x_hat) / C), dw = sum_rows dy x_hat, db = sum_rows dy
 // The column sums stay in registers over the rows that a lane sees, meet in LDS, leave as one row of partial sums per
 // workgroup, and a second kernel adds those in a fixed order: no atomics, reproducible.
-// [262144, 512] bf16: forward 104 to 106 us (5.1 TB/s; a large copy 4.9), backward 138 to 143 (5.6 to 5.85), column sums 4.8.
-// Widths off the 8-column grid pay for accesses that straddle lines: [262144, 257] 87 and 161 us, [262144, 256] 54 and 70.
+// [262144, 512] bf16: forward 101 us (5.3 TB/s; a large copy 4.9), backward 137 to 143 (5.6 to 5.9), column sums 4.8.
+// Widths off the 8-column grid pay for accesses that straddle lines: [262144, 257] 86 and 161 us, [262144, 256] 54 and 70.
 #include "hstu_ffn_common.h"
 
 namespace hstu {
@@ -275,16 +275,20 @@ static LnShape ln_shape(int cols) {
     return s[8];
 }
 static int ln_rows_per_wg(const LnShape& s) { return s.lpr > 256 ? 1 : 256 / s.lpr; }
-// Workgroups that walk down the rows with the next one under way.  Forward: up to 2048 (262144 x 128 fp16: 38 us with a workgroup
-// for every 16 rows, 28 with 2048; 30000 x 2048 bf16: 80 and 56, since a row's weight and bias are loaded once a lane).
+// Workgroups that walk down the rows with the next one under way.  Forward, narrow rows (one piece a lane): up to 2048 (262144 x 128
+// fp16: 38 us with a workgroup for every 16 rows, 27.5 with 2048, 30 with 768).  Wider ones have a row's weight and bias to load before
+// their first: 1024 up to 512 columns (262144 x 512 bf16: 104.6 with 2048, 100.6; 16000 x 512: 10.8 and 8.6; 262144 x 257: 87.3 and 85.9, 103
+// with 768), 768 beyond (16000 x 1000: 20.1 and 16.6; 30000 x 2048: 55 and 48; 3000 x 16384: 66 and 50).
 static unsigned ln_fwd_grid(int64_t rows, const LnShape& s) {
-    const int64_t n = (rows + ln_rows_per_wg(s) - 1) / ln_rows_per_wg(s);
-    return (unsigned)(n < 1 ? 1 : n > 2048 ? 2048 : n);
+    const int64_t n = (rows + ln_rows_per_wg(s) - 1) / ln_rows_per_wg(s), most = s.np == 1 ? 2048 : s.lpr == 32 ? 1024 : 768;
+    return (unsigned)(n < 1 ? 1 : n > most ? most : n);
 }
-// Backward: each one is a row of the partial-sum table too, so no more than fill the chip and two rows a lane at least
-// (262144 x 512 bf16: 148 us with 1024, 137 with 768, 214 with 256; 16384 x 8192: 182, 170 and 146)
+// Backward: each one is a row of the partial-sum table too, so no more than fill the chip and two rows a lane at least, four of wide rows
+// (262144 x 128 fp16: 768 38.7 us, 512 41.9; 262144 x 512 bf16: 768 144, 512 137, 256 146; 30000 x 2048: 512 73, 256 69; 8192 x 4096:
+// 512 52, 256 48; two rows a lane and four, 500 x 4096: 17.1 and 14.6, 7687 x 1000 fp32: 27.0 and 28.6)
 static unsigned ln_bwd_grid(int64_t rows, const LnShape& s) {
-    const int64_t most = s.lpr > 256 ? 256 : s.np > 1 ? 512 : 768, per = 2 * ln_rows_per_wg(s), n = (rows + per - 1) / per;
+    const bool wide = s.lpr >= 256 || s.np == 4;
+    const int64_t most = wide ? 256 : s.np > 1 ? 512 : 768, per = (wide ? 4 : 2) * ln_rows_per_wg(s), n = (rows + per - 1) / per;
     return (unsigned)(n < 1 ? 1 : n > most ? most : n);
 }
 
