@@ -36,7 +36,8 @@ __global__ __launch_bounds__(256) void hstu_pad_rows_kernel(const PadArgs a) {
 // ---- dz ------------------------------------------------------------------------------------------------------------------
 // A lane works on 8 consecutive columns of both halves and walks down its rows; `lanes` lanes side by side, 256 / lanes rows
 // at a time.  HBM-bound: reads d_out and z, writes dz.  Columns [2 f, ld) of dz are set to zero (the product reads them).
-// [16384, 4096] bf16: 805 MB in 140 to 164 us (5.8 to 4.9 TB/s, a large copy 4.9); with z in 8 bits, [16384, 2048], 56 us.  The next row
+// [16384, 4096] bf16: 805 MB in 140 to 153 us (5.8 to 5.3 TB/s, a large copy 4.9); with z in 8 bits, [16384, 2048], 52 us.  dz is stored
+// through the caches, the products read it next (the whole backward 649 us past them, 635 so).  The next row
 // under way while one is worked on was slower (8 bits 45 us for 37 at the time: the registers cost waves).
 struct DzArgs {
     const void* d_out;
