@@ -197,7 +197,8 @@ struct Plan { int tile, splits, tiles_n, tiles_m; int64_t c_split; double us; };
 // beyond one cost a second kernel that adds their fp32 sums.
 // Measured (bf16, a full chip): a piece of a 256 x 256 tile 1.7, of a 256 x 128 one 1.1, of a 128 x 128 one 0.6 alone on its CU with
 // four buffers, 0.65 with two and 1.15 with two workgroups on a CU, of a 64 x 128 one 0.42 and 0.8.  fp32 products are bound by
-// their matrix rate: 128 x 128 x 32 in 1.8, 64 x 128 x 32 in 0.95.
+// their matrix rate: 128 x 128 x 32 in 1.8, 64 x 128 x 32 in 0.95.  Over 129 products of random sizes the choice is 0.3 % (forward), 0.8 %
+// (d_x) and 1.7 % (d_weight) slower than the fastest in the mean, 16 % at worst; fp32 0, 3.5 and 1.2 %.
 // Each tile has the sizes where it is the fastest (forward, us: 256 x 256, 128 x 128, 256 x 128, 64 x 128):
 //   2789 x 1008 x 2736 fp16 37 44 40 55;  16384 x 512 x 2048 bf16 90 91 87 109;  8000 x 128 x 512 bf16 10.4 7.5 7.5 9.0;
 //   256 x 1024 x 4096 bf16 26 12.4 16 9.2;  100 x 2000 x 4000 fp32 473 134 245 74
@@ -217,9 +218,9 @@ static Plan gemm_plan(int kind, int32_t dtype, int64_t M, int64_t N, int64_t C) 
             const bool pairs = (tile == TILE_128 || tile == TILE_64x128) && wgs > 256;   // two workgroups on a CU
             const double piece16[GEMM_TILES] = {1.7, pairs ? 1.15 : 0.65, 0.6, 1.1, pairs ? 0.8 : 0.42};
             const double piece32[GEMM_TILES] = {7.0, pairs ? 3.6 : 1.8, 1.8, 3.5, pairs ? 1.8 : 0.95};
-            const double fixed_us[GEMM_TILES] = {6.0, pairs ? 4.0 : 3.0, 3.0, 4.5, pairs ? 3.0 : 2.5};
+            const double fixed_us[GEMM_TILES] = {6.0, pairs ? 4.0 : 3.0, 4.0, 4.5, pairs ? 3.0 : 2.5};
             const double piece = f32 ? piece32[tile] : piece16[tile], fixed = fixed_us[tile];
-            const double rounds = (double)(int64_t)((wgs + (pairs ? 511 : 255)) / (pairs ? 512 : 256));
+            const double rounds = (double)(int64_t)((wgs + 255) / 256) * (pairs ? 0.5 : 1.0);
             double t = rounds * (fixed + share * piece);
             if (splits > 1) t += 4.0 + (double)splits * M * N * 8 / 4.5e6;
             if (t < least) {
