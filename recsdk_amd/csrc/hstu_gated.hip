@@ -210,6 +210,7 @@ static Plan gemm_plan(int kind, int32_t dtype, int64_t M, int64_t N, int64_t C) 
     Plan best = {};
     double least = 1e300;
     for (int tile = 0; tile < GEMM_TILES; tile++) {   // (the first one also takes what would be too many tiles of the others)
+        if (f32 && tile == TILE_128_DEEP) continue;   // (never the fastest: the copies of two buffers keep ahead of the matrix rate)
         const int64_t tm = (M + gemm_tile_m(tile) - 1) / gemm_tile_m(tile), tn = (N + gemm_tile_n(tile, kind) - 1) / gemm_tile_n(tile, kind);
         for (int splits = 1; splits <= 64; splits *= 2) {
             if (splits > 1 && (kind == GEMM_GATED || pieces < 2 * splits)) break;
@@ -217,7 +218,7 @@ static Plan gemm_plan(int kind, int32_t dtype, int64_t M, int64_t N, int64_t C) 
             const double wgs = (double)tm * tn * splits, share = (double)((pieces + splits - 1) / splits);
             const bool pairs = (tile == TILE_128 || tile == TILE_64x128) && wgs > 256;   // two workgroups on a CU
             const double piece16[GEMM_TILES] = {1.7, pairs ? 1.15 : 0.65, 0.6, 1.1, pairs ? 0.8 : 0.42};
-            const double piece32[GEMM_TILES] = {7.0, pairs ? 3.6 : 1.8, 1.8, 3.5, pairs ? 1.8 : 0.95};
+            const double piece32[GEMM_TILES] = {7.0, pairs ? 3.6 : 1.8, 0.0, 3.5, pairs ? 1.8 : 0.95};
             const double fixed_us[GEMM_TILES] = {6.0, pairs ? 4.0 : 3.0, 4.0, 4.5, pairs ? 3.0 : 2.5};
             const double piece = f32 ? piece32[tile] : piece16[tile], fixed = fixed_us[tile];
             const double rounds = (double)(int64_t)((wgs + 255) / 256) * (pairs ? 0.5 : 1.0);

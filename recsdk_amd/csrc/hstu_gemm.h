@@ -489,7 +489,7 @@ __global__ __launch_bounds__(S::NT) void hstu_gemm_kernel(const GemmArgs a) {
 // kinds of products, and the launchers (one translation unit per element type)
 enum GemmKind : int { GEMM_GATED = 0 /* KC x KC, gated epilogue */, GEMM_DX = 1 /* n side RC, m side KC */, GEMM_DW = 2 /* both RC */ };
 // 256 x 256 outputs by eight waves (one workgroup per CU); 128 x 128 by four, with two buffers (two workgroups per CU) or four (one,
-// whose copies run three pieces ahead); 256 rows m x 128 by eight with three buffers (one); 64 x 128 by four with
+// whose copies run three pieces ahead; 16 bits only); 256 rows m x 128 by eight with three buffers (one); 64 x 128 by four with
 // three (two), for products too small for the others
 enum GemmTile : int { TILE_256 = 0, TILE_128 = 1, TILE_128_DEEP = 2, TILE_256x128 = 3, TILE_64x128 = 4, GEMM_TILES = 5 };
 constexpr int gemm_tile_m(int tile) { return tile == TILE_256 || tile == TILE_256x128 ? 256 : tile == TILE_64x128 ? 64 : 128; }
@@ -506,9 +506,9 @@ template <typename T, bool NRC, bool MRC, int GATE> void launch_gemm_tile(const 
     };
     if (tile == TILE_256) go(GemmShape<T, NRC, MRC, 256, 256, 4, 2, 2, GATE>());
     else if (tile == TILE_128) go(GemmShape<T, NRC, MRC, 128, 128, 2, 2, 2, GATE>());
-    else if (tile == TILE_128_DEEP) go(GemmShape<T, NRC, MRC, 128, 128, 2, 2, 4, GATE>());
     else if (tile == TILE_256x128) go(GemmShape<T, NRC, MRC, 128, 256, 2, 4, 3, GATE>());
-    else go(GemmShape<T, NRC, MRC, 128, 64, 2, 2, 3, GATE>());
+    else if (tile == TILE_64x128) go(GemmShape<T, NRC, MRC, 128, 64, 2, 2, 3, GATE>());
+    else if constexpr (sizeof(T) == 2) go(GemmShape<T, NRC, MRC, 128, 128, 2, 2, 4, GATE>());
 }
 template <typename T> hipError_t launch_gemm_t(const GemmArgs& a, int kind, int tile, hipStream_t st) {
     if (kind == GEMM_DX) launch_gemm_tile<T, true, false, -1>(a, tile, st);

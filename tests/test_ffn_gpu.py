@@ -298,7 +298,14 @@ def test_gated_linear_larger_and_reproducible(m, k, f, dtype, act):
                                                 (8000, 521, 100, BF, "silu", False), (1001, 520, 4000, HF, "silu", False), (8000, 520, 523, BF, "silu", True),
                                                 (4000, 1000, 520, HF, "gelu", False), (4001, 72, 520, BF, "silu", False), (12000, 520, 1000, HF, "silu", False),
                                                 (500, 264, 700, BF, "silu", False), (1000, 520, 2000, HF, "gelu", True), (300, 500, 1500, F32, "silu", False),
-                                                (129, 513, 2047, BF, "gelu", False)])
+                                                (129, 513, 2047, BF, "gelu", False),
+                                                # each tile of fp32, and of the kept formats and activations
+                                                (1094, 16, 3213, F32, "gelu", False), (143, 2000, 3156, F32, "silu", False), (12194, 16, 1803, F32, "silu", False),
+                                                (8247, 130, 33, F32, "gelu", False), (6504, 2000, 32, F32, "silu", False), (6321, 16, 2885, F32, "silu", False),
+                                                (8366, 16, 71, F32, "silu", False), (12810, 256, 194, F32, "gelu", False), (14202, 16, 396, F32, "gelu", False),
+                                                (8764, 2000, 69, HF, "gelu", True), (8764, 2000, 69, BF, "silu", True), (8764, 2000, 69, BF, "gelu", False),
+                                                (11521, 1000, 135, BF, "silu", True), (11521, 1000, 135, HF, "gelu", True), (11521, 1000, 135, HF, "silu", False),
+                                                (500, 264, 700, BF, "gelu", True), (9187, 16, 67, BF, "silu", True), (9497, 16, 392, HF, "gelu", False)])
 def test_gated_linear_every_tile(m, k, f, dtype, act, c8):
     """Sizes at which the products run in each of their tiles, with and without shares of the contraction (64-bit oracle on the GPU)."""
     say("gated_linear tiles", m, k, f, dtype, act, c8)
@@ -322,7 +329,7 @@ def test_gated_linear_every_tile(m, k, f, dtype, act, c8):
 
 
 @pytest.mark.parametrize("m,k,f,dtype",
-                         [(m, k, f, d) for (m, k, f) in ((1, 64, 32), (70, 128, 96), (33, 40, 45), (257, 96, 1000), (600, 512, 256)) for d in (BF, HF)])
+                         [(m, k, f, d) for (m, k, f) in ((1, 64, 32), (70, 128, 96), (33, 40, 45), (257, 96, 1000), (600, 512, 256), (20, 520, 96), (64, 136, 40), (50, 1001, 33)) for d in (BF, HF)])
 def test_gated_linear_checkpoint8(m, k, f, dtype):
     """The forward's result is the one without checkpoints, bit for bit; the codes stand for z within the format's half step; the
     backward is the formula at the values that the codes stand for."""
