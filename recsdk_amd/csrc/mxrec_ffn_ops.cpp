@@ -3,6 +3,7 @@
 // no counterpart in the reference.
 #include <ATen/ATen.h>
 #include <ATen/core/grad_mode.h>
+#include <c10/core/AutogradState.h>
 #include <c10/hip/HIPStream.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
@@ -57,8 +58,15 @@ struct Launch {   // current device and stream of a call
 // an optional tensor argument; undefined where it is missing
 static at::Tensor value(const c10::optional<at::Tensor>& t) { return t.has_value() ? *t : at::Tensor(); }
 
-static void no_double_backward(const char* op) {
+// Forward-mode derivatives are not implemented, and a result without a tangent counts as a constant: inputs that carry one are refused
+// (not where forward mode is switched off, as in the forward of a caller's own autograd function).
+static void no_tangents(const char* op, std::initializer_list<const at::Tensor*> ts) {
+    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+    for (const at::Tensor* t : ts) TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), op, ": forward-mode derivatives are not supported (an input carries a tangent)");
+}
+static void no_double_backward(const char* op, const at::Tensor& grad) {
     TORCH_CHECK(!at::GradMode::is_enabled(), op, ": the backward is not differentiable (called with create_graph=True)");
+    no_tangents(op, {&grad});
 }
 
 // ---- layer_norm --------------------------------------------------------------------------------------------------------
@@ -91,6 +99,7 @@ static at::ScalarType ln_param_type(const at::Tensor& x, const at::Tensor& weigh
 // {y} or {y, mean, rstd}
 static std::vector<at::Tensor> ln_forward(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& bias, double eps, bool stats) {
     ln_check(x, weight, bias, eps);
+    no_tangents(LN, {&x, &weight, &bias});
     check_devices(LN, {&x, &weight, &bias});
     Launch launch(x);
     const at::Tensor xr = rows_of(x), w = weight.defined() ? weight.contiguous() : weight, b = bias.defined() ? bias.contiguous() : bias;
@@ -175,7 +184,7 @@ public:
         return outs[0];
     }
     static torch::autograd::tensor_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::tensor_list grads) {
-        no_double_backward(LN);
+        no_double_backward(LN, grads[0]);
         const auto s = ctx->get_saved_variables();
         const auto pt = (at::ScalarType)ctx->saved_data["param_type"].toInt();
         const bool hw = ctx->saved_data["has_weight"].toBool(), hb = ctx->saved_data["has_bias"].toBool();
@@ -197,6 +206,7 @@ at::Tensor layer_norm(const at::Tensor& x, const c10::optional<at::Tensor>& weig
 }
 at::Tensor layer_norm_autograd(const at::Tensor& x, const c10::optional<at::Tensor>& weight, const c10::optional<at::Tensor>& bias, double eps) {
     const at::Tensor w = value(weight), b = value(bias);
+    no_tangents(LN, {&x, &w, &b});
     if (!wants_grad({&x, &w, &b})) {
         at::AutoDispatchBelowADInplaceOrView guard;
         return ln_forward(x, w, b, eps, false)[0];
@@ -210,6 +220,7 @@ std::vector<at::Tensor> layer_norm_backward(const at::Tensor& d_out, const at::T
                                             const at::Tensor& rstd) {
     const at::Tensor w = value(weight);
     ln_check(x, w, at::Tensor(), 1.0);
+    no_tangents(LN, {&d_out, &x, &w, &mean, &rstd});
     TORCH_CHECK(d_out.sizes() == x.sizes() && d_out.scalar_type() == x.scalar_type(), LN, ": d_out must have the shape and dtype of x");
     const int64_t rows = row_count(x);
     for (const at::Tensor* t : {&mean, &rstd})
@@ -263,6 +274,7 @@ static Kept kept_like(const at::Tensor& x, int64_t f, bool checkpoint8) {
 // {out}, {out, z} (fp32), {out, upper parts of z, lower parts} (16-bit types: z in 24 bits) or {out, codes, exponents}
 static std::vector<at::Tensor> gl_forward(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& bias, int32_t act, int32_t keep) {
     gl_check(x, weight, bias, keep == HSTU_KEEP_8BIT);
+    no_tangents(GL, {&x, &weight, &bias});
     check_devices(GL, {&x, &weight, &bias});
     Launch launch(x);
     const at::Tensor xr = rows_of(x), w = weight.contiguous(), b = bias.defined() ? bias.contiguous() : bias;
@@ -355,7 +367,7 @@ public:
         return outs[0];
     }
     static torch::autograd::tensor_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::tensor_list grads) {
-        no_double_backward(GL);
+        no_double_backward(GL, grads[0]);
         const auto s = ctx->get_saved_variables();
         auto g = gl_backward(grads[0], s[0], s[1], s[2], s[3], (int32_t)ctx->saved_data["act"].toInt(), (at::ScalarType)ctx->saved_data["bias_type"].toInt(),
                              ctx->needs_input_grad(0), ctx->needs_input_grad(1), ctx->saved_data["has_bias"].toBool() && ctx->needs_input_grad(2));
@@ -370,6 +382,7 @@ at::Tensor gated_linear(const at::Tensor& x, const at::Tensor& weight, const c10
 at::Tensor gated_linear_autograd(const at::Tensor& x, const at::Tensor& weight, const c10::optional<at::Tensor>& bias, c10::string_view activation,
                                  bool checkpoint8) {
     const at::Tensor b = value(bias);
+    no_tangents(GL, {&x, &weight, &b});
     if (!wants_grad({&x, &weight, &b})) {
         at::AutoDispatchBelowADInplaceOrView guard;
         return gated_linear(x, weight, bias, activation, checkpoint8);
@@ -385,6 +398,7 @@ std::vector<at::Tensor> gated_linear_backward(const at::Tensor& d_out, const at:
     const at::Tensor aux = value(z_aux);
     const bool c8 = z.scalar_type() == at::kFloat8_e4m3fn;
     gl_check(x, weight, at::Tensor(), c8);
+    no_tangents(GL, {&d_out, &x, &weight, &z});
     const int64_t f = weight.size(0) / 2;
     const Kept k = kept_like(x, f, c8);
     TORCH_CHECK(d_out.scalar_type() == x.scalar_type() && d_out.sizes().vec() == with_last(x, f), GL, ": d_out must have the dtype of x and the shape of out");
@@ -413,6 +427,7 @@ std::vector<at::Tensor> activation_pack8(const at::Tensor& x) {
     TORCH_CHECK(x.defined() && x.dim() >= 1, op, ": x must have at least 1 dimension");
     const int64_t rows = row_count(x), cols = x.size(-1);
     hstu_pack8_params p = pack8_params(op, x.scalar_type(), rows, cols);
+    no_tangents(op, {&x});
     check_devices(op, {&x});
     Launch launch(x);
     const at::Tensor xr = rows_of(x);
@@ -435,6 +450,7 @@ at::Tensor activation_unpack8(const at::Tensor& codes, const at::Tensor& exponen
     TORCH_CHECK(exponents.scalar_type() == at::kByte && exponents.sizes().vec() == with_last(codes, (cols + HSTU_PACK8_GROUP - 1) / HSTU_PACK8_GROUP), op,
                 ": exponents must be uint8 with the shape of codes and ceil(", cols, " / 32) values along the last dimension, but get ", exponents.scalar_type(), " ",
                 exponents.sizes());
+    no_tangents(op, {&codes});
     check_devices(op, {&codes, &exponents});
     Launch launch(codes);
     const at::Tensor cc = codes.contiguous(), ec = exponents.contiguous();
