@@ -24,7 +24,8 @@ extern "C" {
 
 /* LayerNorm over the last axis:
  *   y = x_hat * weight + bias     x_hat = (x - mean) * rstd     rstd = 1 / sqrt(var + eps)
- * mean and (biased) variance in fp32, the variance from the deviations; y rounded once.  rows may be 0. */
+ * mean and (biased) variance in fp32, the variance from the deviations; y rounded once.  Finite rows of any size are taken (up to
+ * 2^126: beyond it a deviation itself may leave fp32); a row with a NaN or an infinity has NaN for y, mean and rstd.  rows may be 0. */
 typedef struct hstu_layer_norm_params {
     uint32_t struct_size;
     int32_t dtype;         /* HSTU_F32 / HSTU_F16 / HSTU_BF16: x, y */

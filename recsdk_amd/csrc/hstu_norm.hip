@@ -67,6 +67,32 @@ template <typename T> __device__ __forceinline__ void ln_param(const void* p, bo
     }
 }
 
+// A row's sum is formed in units of this power of two, as many as there can be columns: it stays in fp32 for every row that does
+constexpr float LN_SUM_UNIT = (float)HSTU_LN_MAX_COLS;
+static_assert(HSTU_LN_MAX_COLS == 1 << 14, "a power of two");
+
+// rstd of a row whose squared deviations `v` leave fp32 (the largest of them then is 2^57 or more): from deviations in units of 2^90,
+// and `rest`, their mean.  NaN where one of them is no number
+template <int LPR, int NP> __device__ __forceinline__ float ln_far_rstd(const float (&v)[NP][8], int l, int cols, float eps, float* red, float& rest) {
+    constexpr float UNIT = 0x1p90f, INV = 0x1p-90f;
+    const float count = (float)cols;
+    float d1 = 0.f, d2 = 0.f;
+#pragma unroll
+    for (int q = 0; q < NP; q++)
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const float d = (q * LPR + l) * 8 + k < cols ? v[q][k] * INV : 0.f;
+            d1 += d;
+            d2 += d * d;
+        }
+    ln_sum<LPR>(d1, d2, red, 0);
+    if constexpr (LPR > 64) __syncthreads();   // (the next row's first sum takes the same place in LDS)
+    const float r = d1 / count, t = d2 / count - r * r, var = t < 0.f ? 0.f : t;
+    rest = r * UNIT;
+    // the variance itself, UNIT^2 var, fits where it is small: only there may eps be all that is left
+    return var > 0x1p-100f ? INV / sqrtf(var + eps * INV * INV) : 1.0f / sqrtf(var * UNIT * UNIT + eps);
+}
+
 template <typename T, int LPR, int NP>
 __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void hstu_layer_norm_fwd_kernel(const hstu_layer_norm_params p) {
     constexpr int NT = LPR > 256 ? LPR : 256, RPW = NT / LPR;
@@ -100,11 +126,11 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void hstu_layer_norm_fwd_ker
 #pragma unroll
         for (int q = 0; q < NP; q++)
 #pragma unroll
-            for (int k = 0; k < 8; k++) s += v[q][k];
+            for (int k = 0; k < 8; k++) s = __builtin_fmaf(v[q][k], 1.0f / LN_SUM_UNIT, s);
         ln_sum<LPR>(s, none, red, 0);
         // deviations from the rounded mean, and from them what rounding took from it: rows far from zero keep their accuracy
         // (a constant row has x_hat = 0, not the rounding of its mean times 1 / sqrt(eps))
-        const float near = s / count;
+        const float near = s / count * LN_SUM_UNIT;
         float d1 = 0.f, d2 = 0.f;
 #pragma unroll
         for (int q = 0; q < NP; q++)
@@ -117,8 +143,10 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void hstu_layer_norm_fwd_ker
                 d2 += in ? d * d : 0.f;
             }
         ln_sum<LPR>(d1, d2, red, 1);
-        const float rest = d1 / count, mean = near + rest;
-        const float rstd = 1.0f / sqrtf(fmaxf(d2 / count - rest * rest, 0.f) + p.eps);
+        float rest = d1 / count, rstd;
+        if (d2 <= 3.4e38f) rstd = 1.0f / sqrtf(fmaxf(d2 / count - rest * rest, 0.f) + p.eps);
+        else rstd = ln_far_rstd<LPR, NP>(v, l, p.cols, p.eps, red, rest);
+        const float mean = near + rest;
         if (l == 0 && p.mean) { p.mean[row] = mean; p.rstd[row] = rstd; }
         T* y = reinterpret_cast<T*>(p.y) + row * p.cols;
 #pragma unroll

@@ -5,9 +5,47 @@ import torch
 import torch.autograd.forward_ad as fwd_ad
 
 import recsdk_amd  # noqa: F401
-from tests.test_ffn_gpu import BF, EPS, M, say
+from oracle import ffn_oracle as FO
+from tests.test_ffn_gpu import BF, EPS, F32, M, ln_case, ln_tolerances, say, within
 
 pytestmark = pytest.mark.gpu
+
+
+# ---- layer_norm: extreme rows ----------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("cols", [2, 7, 64, 300, 512, 1000, 2048, 3000, 5000, 16384])
+@pytest.mark.parametrize("dtype,scale", [(BF, 2.0 ** 62), (BF, 2.0 ** 90), (F32, 2.0 ** 64), (F32, 2.0 ** 110), (F32, 2.0 ** 120)])
+def test_layer_norm_rows_whose_squares_leave_fp32(cols, dtype, scale):
+    """Finite rows whose squared deviations are beyond fp32, among ordinary ones: mean, rstd, y and the gradients as for any row."""
+    say("large rows", cols, dtype, scale)
+    x, w, b, dy = ln_case(6, cols, dtype, dtype, cols)
+    x[1] *= scale
+    x[4] = x[4].abs() * scale + scale
+    y0, mean, rstd = FO.layer_norm(x, w, b, EPS)
+    t = ln_tolerances(x, w, b, dy, dtype, (mean, rstd))
+    y, mn, rs = M.layer_norm_forward(x.cuda(), w.cuda(), b.cuda(), EPS)
+    assert torch.equal(M.layer_norm(x.cuda(), w.cuda(), b.cuda(), EPS), y)
+    # a result in fp32's subnormal range has a fixed step of 2^-149
+    within(mn, mean, t[1], "mean")
+    within(rs, rstd, t[2] + 2.0 ** -149, "rstd")
+    within(y, y0, t[0], "y")
+    dx, dw, _ = M.layer_norm_backward(dy.cuda(), x.cuda(), w.cuda(), mn, rs)
+    want = FO.layer_norm_backward(dy, x, w, mean, rstd)
+    within(dx, want[0], t[3] + 2.0 ** -149, "d_x")
+    within(dw, want[1], t[4], "d_weight")
+
+
+@pytest.mark.parametrize("cols", [5, 300, 1000, 5000])
+def test_layer_norm_statistics_of_rows_with_nan_or_infinity(cols):
+    """mean and rstd of such a row are NaN, and so is its d_x; the other rows keep theirs."""
+    x, w, b, dy = ln_case(6, cols, F32, F32, 3)
+    clean = M.layer_norm_forward(x.cuda(), w.cuda(), b.cuda(), EPS)
+    dclean = M.layer_norm_backward(dy.cuda(), x.cuda(), w.cuda(), *clean[1:])[0]
+    x[1, cols - 1], x[3, 0], x[4, cols // 2] = float("nan"), float("inf"), -float("inf")
+    got = M.layer_norm_forward(x.cuda(), w.cuda(), b.cuda(), EPS)
+    dx = M.layer_norm_backward(dy.cuda(), x.cuda(), w.cuda(), *got[1:])[0]
+    for a, c in zip([*got, dx], [*clean, dclean]):
+        assert torch.equal(a[[0, 2, 5]], c[[0, 2, 5]]) and bool(torch.isnan(a[[1, 3, 4]]).all())
 
 
 # ---- forward-mode tangents ---------------------------------------------------------------------------------------------------
