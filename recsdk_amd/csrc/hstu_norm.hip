@@ -204,10 +204,12 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void hstu_layer_norm_bwd_ker
         if (AHEAD && row + step < p.rows) fetch(row + step);
         float s1 = 0.f, s2 = 0.f;
 #pragma unroll
-        for (int q = 0; q < NP; q++)
+        for (int q = 0; q < NP; q++) {
+            const int left = p.cols - (q * LPR + l) * 8;
 #pragma unroll
             for (int k = 0; k < 8; k++) {
-                xh[q][k] = (xh[q][k] - mean) * rstd;   // columns behind the row have g = 0
+                // (behind the row both are zero: -mean * rstd may be infinite)
+                xh[q][k] = k < left ? (xh[q][k] - mean) * rstd : 0.f;
                 gw[q][k] += g[q][k] * xh[q][k];
                 gb[q][k] += g[q][k];
                 const float a = g[q][k] * w[q][k];
@@ -215,6 +217,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void hstu_layer_norm_bwd_ker
                 s1 += a;
                 s2 += a * xh[q][k];
             }
+        }
         if (p.d_x) {
             ln_sum<LPR>(s1, s2, red, slot);
             slot ^= 1;

@@ -6,12 +6,42 @@ import torch.autograd.forward_ad as fwd_ad
 
 import recsdk_amd  # noqa: F401
 from oracle import ffn_oracle as FO
-from tests.test_ffn_gpu import BF, EPS, F32, M, ln_case, ln_tolerances, say, within
+from tests.test_ffn_gpu import BF, E32, EPS, F32, M, TINY, U, ln_case, ln_tolerances, say, within
 
 pytestmark = pytest.mark.gpu
 
 
 # ---- layer_norm: extreme rows ----------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("cols", [1, 7, 8, 63, 64, 250, 300, 512, 1000, 1500, 2049, 5000, 16000, 16384])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_layer_norm_backward_of_large_constant_rows(cols, dtype):
+    """A constant row has x_hat = 0 whatever its size, also where mean * rstd is beyond fp32, and whatever part of the lanes the row
+    fills: d_x = rstd (a - mean(a)), the rows beside it as ever."""
+    say("large constant rows", cols, dtype)
+    x, w, b, dy = ln_case(5, cols, dtype, dtype, cols)
+    x[1], x[3] = 2.0 ** 120, -2.0 ** 114                     # (the mean of a power of two is exact)
+    _, mean, rstd = FO.layer_norm(x, w, b, EPS)
+    t = ln_tolerances(x, w, b, dy, dtype, (mean, rstd))
+    y, mn, rs = M.layer_norm_forward(x.cuda(), w.cuda(), b.cuda(), EPS)
+    assert torch.equal(y[1].cpu(), b) and torch.equal(y[3].cpu(), b)
+    assert float(mn[1]) == 2.0 ** 120 and float(mn[3]) == -2.0 ** 114
+    dx, dw, db = M.layer_norm_backward(dy.cuda(), x.cuda(), w.cuda(), mn, rs)
+    want = FO.layer_norm_backward(dy, x, w, mean, rstd)
+    assert bool(torch.isfinite(dx).all()) and bool(torch.isfinite(dw).all())
+    keep = [0, 2, 4]
+    within(dx[keep], want[0][keep], t[3][keep], "d_x")
+    # x_hat is exactly 0: the tolerance of the others, whose terms in x_hat are relative to |x|, is far too wide here
+    for r in (1, 3):
+        a = dy[r].double() * w.double()
+        inner = 58 * E32 * a.abs().mean() + 6 * E32 * (a.abs() + a.mean().abs())
+        within(dx[r], want[0][r], U[dtype] * want[0][r].abs() + TINY[dtype] + rstd[r] * inner + 66 * E32 * want[0][r].abs(), "d_x of a constant row")
+    g, xh = dy[keep].double(), (x[keep].double() - mean[keep, None]) * rstd[keep, None]
+    ref = (g * xh).sum(dim=0)
+    tk = ln_tolerances(x[keep], w, b, dy[keep], dtype, (mean[keep], rstd[keep]))
+    within(dw, ref, tk[4], "d_weight")
+    within(db, want[2], (64 + 40 + 1) * E32 * dy.double().abs().sum(dim=0), "d_bias")
+
 
 @pytest.mark.parametrize("cols", [2, 7, 64, 300, 512, 1000, 2048, 3000, 5000, 16384])
 @pytest.mark.parametrize("dtype,scale", [(BF, 2.0 ** 62), (BF, 2.0 ** 90), (F32, 2.0 ** 64), (F32, 2.0 ** 110), (F32, 2.0 ** 120)])
