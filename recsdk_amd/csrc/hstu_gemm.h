@@ -439,9 +439,14 @@ __global__ __launch_bounds__(S::NT) void hstu_gemm_kernel(const GemmArgs a) {
                 zg[r] = acc[gb][j][r] + bg[r];
                 zu[r] = acc[NB / 2 + gb][j][r] + bu[r];
             }
-            // kept rows hold whole blocks; columns past f hold zero (no weight row, no bias)
+            // kept rows hold whole blocks, with zeros past f: their products are 0 * x, NaN for a row with a NaN or an infinity
             const int64_t kept = HSTU_GATED_KEPT((int64_t)a.N);
             const int whole = left > 0 ? 32 : 0;
+            if (S::KEEP != HSTU_KEEP_NONE && n + 32 > a.N) {
+#pragma unroll
+                for (int r = 0; r < 16; r++)
+                    if (n + 8 * (r >> 2) + 4 * g + (r & 3) >= a.N) zg[r] = zu[r] = 0.f;
+            }
             if constexpr (S::KEEP == HSTU_KEEP_FULL && S::ES == 4) {
 #pragma unroll
                 for (int part = 0; part < 2; part++) store_block<T>(reinterpret_cast<T*>(a.z) + (m * 2 + part) * kept + n, part ? zu : zg, g, whole);

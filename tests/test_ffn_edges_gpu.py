@@ -6,7 +6,7 @@ import torch.autograd.forward_ad as fwd_ad
 
 import recsdk_amd  # noqa: F401
 from oracle import ffn_oracle as FO
-from tests.test_ffn_gpu import BF, E32, EPS, F32, M, TINY, U, ln_case, ln_tolerances, say, within
+from tests.test_ffn_gpu import BF, E32, EPS, F32, HF, M, TINY, U, gl_case, ln_case, ln_tolerances, say, within
 
 pytestmark = pytest.mark.gpu
 
@@ -76,6 +76,27 @@ def test_layer_norm_statistics_of_rows_with_nan_or_infinity(cols):
     dx = M.layer_norm_backward(dy.cuda(), x.cuda(), w.cuda(), *got[1:])[0]
     for a, c in zip([*got, dx], [*clean, dclean]):
         assert torch.equal(a[[0, 2, 5]], c[[0, 2, 5]]) and bool(torch.isnan(a[[1, 3, 4]]).all())
+
+
+# ---- gated_linear: what is kept behind the last column ------------------------------------------------------------------------
+
+@pytest.mark.parametrize("m,k,f", [(5, 64, 45), (40, 1000, 300), (200, 70, 90), (300, 96, 33), (2000, 640, 2001), (4000, 48, 129)])
+@pytest.mark.parametrize("dtype,c8", [(BF, False), (HF, True), (HF, False), (BF, True), (F32, False)])
+def test_gated_linear_keeps_zeros_behind_the_columns(m, k, f, dtype, c8):
+    """Also for rows of x with a NaN or an infinity, whichever kernel runs."""
+    say("kept zeros", m, k, f, dtype, c8)
+    x, w, b, _ = (t.cuda() for t in gl_case(m, k, f, dtype, True, 13))
+    x[1, 0], x[m - 1, k - 1], x[m // 2, k // 2] = float("nan"), float("inf"), -float("inf")
+    _, z, *aux = M.gated_linear_forward(x, w, b, "silu", c8)
+    fp = (f + 31) // 32 * 32
+    if not c8 and dtype != F32:
+        z = z.transpose(1, 2).reshape(m, 2, fp)
+    assert z.shape == (m, 2, fp)
+    raw = {1: torch.uint8, 2: torch.int16, 4: torch.int32}[z.element_size()]
+    assert not bool(z.contiguous().view(raw)[:, :, f:].any())
+    if not c8 and aux:
+        assert not bool(aux[0][:, :, f:].any())
+    assert bool(torch.isnan(z[1, :, :f].float()).all())
 
 
 # ---- forward-mode tangents ---------------------------------------------------------------------------------------------------
