@@ -154,6 +154,12 @@ typedef struct hstu_gated_bwd_params {
 int hstu_hip_gated_linear_backward_get_workspace_size(const hstu_gated_bwd_params* p, uint64_t* workspace_bytes);
 int hstu_hip_gated_linear_backward(const hstu_gated_bwd_params* p, void* workspace, uint64_t workspace_bytes, void* stream);
 
+/* Which kernels the given arguments select, NUL-terminated into buf; nothing is launched.  Forward: "rows_bf16_48" (few rows: the
+ * instance for up to 48) or "tiles_bf16_256x128" (rows x columns of z, "_deep": four buffers).  Backward: both products with the number
+ * of shares of their contraction, "dx_f16_256x128_1 dw_f16_128x128_deep_4". */
+int hstu_hip_gated_linear_describe_kernel(const hstu_gated_params* p, char* buf, size_t buf_bytes);
+int hstu_hip_gated_linear_backward_describe_kernel(const hstu_gated_bwd_params* p, char* buf, size_t buf_bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -36,6 +36,7 @@ EXPORTS = [
     "hstu_hip_activation_pack8", "hstu_hip_activation_unpack8",
     "hstu_hip_gated_linear", "hstu_hip_gated_linear_get_workspace_size",
     "hstu_hip_gated_linear_backward", "hstu_hip_gated_linear_backward_get_workspace_size",
+    "hstu_hip_gated_linear_describe_kernel", "hstu_hip_gated_linear_backward_describe_kernel",
 ]
 
 
@@ -230,6 +231,8 @@ def lib() -> C.CDLL:
         for n, t in (("layer_norm_backward", HstuLayerNormBwdParams), ("gated_linear", HstuGatedParams), ("gated_linear_backward", HstuGatedBwdParams)):
             getattr(_lib, f"hstu_hip_{n}").argtypes = [C.POINTER(t), C.c_void_p, C.c_uint64, C.c_void_p]
             getattr(_lib, f"hstu_hip_{n}_get_workspace_size").argtypes = [C.POINTER(t), C.POINTER(C.c_uint64)]
+        _lib.hstu_hip_gated_linear_describe_kernel.argtypes = [C.POINTER(HstuGatedParams), C.c_char_p, C.c_size_t]
+        _lib.hstu_hip_gated_linear_backward_describe_kernel.argtypes = [C.POINTER(HstuGatedBwdParams), C.c_char_p, C.c_size_t]
         _lib.hstu_hip_kv_token_positions.argtypes = [C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p]
     return _lib
 
@@ -359,4 +362,12 @@ def describe_backward_kernel(params: HstuBwdParams) -> str:
 def describe_kernel(params: HstuFwdParams) -> str:
     buf = C.create_string_buffer(64)
     _check(lib().hstu_hip_describe_kernel(C.byref(params), buf, 64))
+    return buf.value.decode()
+
+
+def describe_gated_linear(params) -> str:
+    """Kernels that ``HstuGatedParams`` or ``HstuGatedBwdParams`` select."""
+    buf = C.create_string_buffer(96)
+    fn = lib().hstu_hip_gated_linear_describe_kernel if isinstance(params, HstuGatedParams) else lib().hstu_hip_gated_linear_backward_describe_kernel
+    _check(fn(C.byref(params), buf, 96))
     return buf.value.decode()

@@ -6,6 +6,8 @@
 //             which read their operands as they lie in memory (transposing LDS reads; nothing is transposed in HBM)
 // dz is rounded to the I/O type between the two: the products run on the 16-bit matrix cores, and the rounding (2^-9 relative
 // per element, independent) averages out over sums of 2 f and of m terms.
+#include <cstdio>
+
 #include "hstu_ffn_common.h"
 #include "hstu_gated_rows.h"
 
@@ -473,6 +475,29 @@ extern "C" int hstu_hip_gated_linear(const hstu_gated_params* p, void* workspace
         e = launch_gemm(p->dtype, a, GEMM_GATED, pl.tile, st);
     }
     if (e != hipSuccess) return fail(HSTU_ERR_LAUNCH, "kernel launch failed: %s", hipGetErrorString(e));
+    return HSTU_OK;
+}
+
+static const char* const TYPE_NAMES[3] = {"f32", "f16", "bf16"};
+static const char* const TILE_NAMES[GEMM_TILES] = {"256x256", "128x128", "128x128_deep", "256x128", "64x128"};
+static_assert(HSTU_F32 == 0 && HSTU_F16 == 1 && HSTU_BF16 == 2, "in the order of TYPE_NAMES");
+
+extern "C" int hstu_hip_gated_linear_describe_kernel(const hstu_gated_params* p, char* buf, size_t n) {
+    if (!buf || n == 0) return fail(HSTU_ERR_INVALID_ARGUMENT, "buf is NULL");
+    const int rc = gated_validate(p);
+    if (rc != HSTU_OK) return rc;
+    if (p->m > 0 && few_rows(p)) snprintf(buf, n, "rows_%s_%d", TYPE_NAMES[p->dtype], (int)(p->m + 15) / 16 * 16);
+    else snprintf(buf, n, "tiles_%s_%s", TYPE_NAMES[p->dtype], TILE_NAMES[gemm_plan(GEMM_GATED, p->dtype, p->m, p->f, p->k).tile]);
+    return HSTU_OK;
+}
+
+extern "C" int hstu_hip_gated_linear_backward_describe_kernel(const hstu_gated_bwd_params* p, char* buf, size_t n) {
+    if (!buf || n == 0) return fail(HSTU_ERR_INVALID_ARGUMENT, "buf is NULL");
+    const int rc = gated_bwd_validate(p);
+    if (rc != HSTU_OK) return rc;
+    const GatedBwdLayout l = gated_bwd_layout(p);
+    const char* t = TYPE_NAMES[p->dtype];
+    snprintf(buf, n, "dx_%s_%s_%d dw_%s_%s_%d", t, TILE_NAMES[l.dx.tile], l.dx.splits, t, TILE_NAMES[l.dw.tile], l.dw.splits);
     return HSTU_OK;
 }
 

@@ -6,7 +6,9 @@ import torch.autograd.forward_ad as fwd_ad
 
 import recsdk_amd  # noqa: F401
 from oracle import ffn_oracle as FO
-from tests.test_ffn_gpu import BF, E32, EPS, F32, HF, M, TINY, U, gl_case, ln_case, ln_tolerances, say, within
+from tests.ffn_cases import INSTANCES
+from tests.test_ffn_gpu import (BF, CUT, E32, EPS, F32, HF, M, TINY, U, gl_backward_tol, gl_case, gl_forward_tol, joined, ln_case, ln_tolerances, say,
+                                within)
 
 pytestmark = pytest.mark.gpu
 
@@ -97,6 +99,44 @@ def test_gated_linear_keeps_zeros_behind_the_columns(m, k, f, dtype, c8):
     if not c8 and aux:
         assert not bool(aux[0][:, :, f:].any())
     assert bool(torch.isnan(z[1, :, :f].float()).all())
+
+
+# ---- gated_linear: every instance ------------------------------------------------------------------------------------------------
+
+def near(got, want, tol, what):
+    """`within`, where the tensors are."""
+    bad = ~((got.double() - want.double()).abs() <= tol)
+    assert got.shape == want.shape and not bool(bad.any()), f"{what}: {int(bad.sum())} of {bad.numel()} out"
+
+
+@pytest.mark.parametrize("m,k,f", INSTANCES)
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+def test_gated_linear_every_instance(m, k, f, dtype):
+    """Serving, and training with each kept format, with each activation, in every kernel that the products have: one forward result,
+    bit for bit, which is the oracle's; what is kept stands for z; the gradients are the formula's at what is kept."""
+    for act in ("silu", "gelu"):
+        say("every instance", m, k, f, dtype, act)
+        x, w, b, do = (t.cuda() for t in gl_case(m, k, f, dtype, True, 17 * m + f))
+        out0, z0 = FO.gated_linear(x, w, b, act)
+        tz, to = gl_forward_tol(x, w, b, z0, act, dtype)
+        served = M.gated_linear(x, w, b, act)
+        near(served, out0, to, "out")
+        del out0, to
+        for c8 in (False, True) if dtype != F32 else (False,):
+            out, z, *aux = M.gated_linear_forward(x, w, b, act, c8)
+            assert torch.equal(out, served)
+            if c8:
+                vals, exps = z.float().double()[:, :, :f], aux[0]
+                unit = torch.ldexp(torch.ones(exps.shape, dtype=torch.float64, device="cuda"), exps.to(torch.int64) - 127).repeat_interleave(32, dim=2)[:, :, :f]
+                zk, unit = (vals * unit).reshape(m, 2 * f).float(), unit.reshape(m, 2 * f)
+                near(zk, z0, torch.maximum((z0.abs() + tz) * 2.0 ** -4, unit * 2.0 ** -10) + tz, "held z")
+            else:
+                zk = joined(f, z, *aux).cuda()
+                near(zk, z0, tz + (U[F32] + CUT[dtype]) * z0.abs() + TINY[F32], "z")
+            got = M.gated_linear_backward(do, x, w, z, *aux, activation=act)
+            *want, dz = FO.gated_linear_backward(do, x, w, zk, act)
+            for a, r, t, n in zip(got, want, gl_backward_tol(do, x, w, zk, act, dtype, dtype, dz), ("d_x", "d_weight", "d_bias")):
+                near(a, r, t, n)
 
 
 # ---- forward-mode tangents ---------------------------------------------------------------------------------------------------
