@@ -139,6 +139,97 @@ def test_gated_linear_every_instance(m, k, f, dtype):
                 near(a, r, t, n)
 
 
+# ---- far offsets and largest sizes -----------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("c8", [False, True])
+def test_d_weight_and_d_bias_over_rows_beyond_32_bits(c8):
+    """dz and z have more than 2^31 elements; only rows at the start, across the middle and at the end have an upstream gradient, so that
+    d_weight and d_bias are those of these rows alone."""
+    k, f = 16, 4096
+    m = (1 << 31) // (2 * f) + 500
+    say("far rows of d_weight", m, k, f, c8)
+    x = torch.randn(m, k, device="cuda", generator=torch.Generator("cuda").manual_seed(1)).to(BF)
+    w = (torch.randn(2 * f, k, device="cuda", generator=torch.Generator("cuda").manual_seed(2)) / 4).to(BF)
+    rows = torch.cat([torch.arange(0, 70), torch.arange(m // 2 - 40, m // 2 + 40), torch.arange(m - 640, m)]).cuda()
+    do = torch.zeros(m, f, dtype=BF, device="cuda")
+    do[rows] = torch.randn(len(rows), f, device="cuda", generator=torch.Generator("cuda").manual_seed(3)).to(BF)
+    _, z, aux = M.gated_linear_forward(x, w, None, "silu", c8)
+    got = M.gated_linear_backward(do, x, w, z, aux)
+    if c8:
+        unit = torch.ldexp(torch.ones(len(rows), 2, f // 32, dtype=torch.float64, device="cuda"), aux[rows].to(torch.int64) - 127).repeat_interleave(32, dim=2)
+        zk = (z[rows].float().double() * unit).reshape(len(rows), 2 * f).float()
+    else:
+        zk = joined(f, z[rows], aux[rows]).cuda()
+    *want, dz = FO.gated_linear_backward(do[rows], x[rows], w, zk, "silu")
+    tols = gl_backward_tol(do[rows], x[rows], w, zk, "silu", BF, BF, dz)
+    near(got[0][rows], want[0], tols[0], "d_x")
+    rest = torch.ones(m, dtype=torch.bool, device="cuda")
+    rest[rows] = False
+    assert not bool(got[0][rest].any())
+    near(got[1], want[1], tols[1], "d_weight")
+    near(got[2], want[2], tols[2], "d_bias")
+
+
+@pytest.mark.parametrize("m,dtype,c8", [(5, BF, False), (70, HF, True), (300, BF, False)])
+def test_gated_linear_at_its_largest_sizes(m, dtype, c8):
+    """k = 16384, f = 32768: weight and d_weight of 2^30 elements."""
+    k, f = 16384, 32768
+    say("largest sizes", m, k, f, dtype, c8)
+    g = torch.Generator("cuda").manual_seed(5)
+    rnd = lambda *s, std=1.0: (torch.randn(*s, device="cuda", generator=g) * std).to(dtype)
+    x, w, b, do = rnd(m, k), rnd(2 * f, k, std=k ** -0.5), rnd(2 * f, std=0.2), rnd(m, f)
+    out0, z0 = FO.gated_linear(x, w, b, "silu")
+    tz, to = gl_forward_tol(x, w, b, z0, "silu", dtype)
+    out, z, *aux = M.gated_linear_forward(x, w, b, "silu", c8)
+    near(out, out0, to, "out")
+    assert torch.equal(M.gated_linear(x, w, b), out)
+    if c8:
+        unit = torch.ldexp(torch.ones(aux[0].shape, dtype=torch.float64, device="cuda"), aux[0].to(torch.int64) - 127).repeat_interleave(32, dim=2)
+        zk = (z.float().double() * unit).reshape(m, 2 * f).float()
+    else:
+        zk = joined(f, z, *aux).cuda()
+        near(zk, z0, tz + (U[F32] + CUT[dtype]) * z0.abs() + TINY[F32], "z")
+    got = M.gated_linear_backward(do, x, w, z, *aux)
+    *want, dz = FO.gated_linear_backward(do, x, w, zk, "silu")
+    for a, r, t, n in zip(got, want, gl_backward_tol(do, x, w, zk, "silu", dtype, dtype, dz), ("d_x", "d_weight", "d_bias")):
+        near(a, r, t, n)
+
+
+@pytest.mark.parametrize("cols", [65536, 65535, 65505])
+def test_pack8_of_the_widest_rows(cols):
+    """What pieces of whole groups give, bit for bit."""
+    x = (torch.randn(37, cols, generator=torch.Generator().manual_seed(cols)) * 3).to(BF).cuda()
+    codes, exps = M.activation_pack8(x)
+    back = M.activation_unpack8(codes, exps, BF)
+    for lo in range(0, cols, 8192):
+        hi = min(lo + 8192, cols)
+        c, e = M.activation_pack8(x[:, lo:hi])
+        assert torch.equal(codes[:, lo:hi].view(torch.uint8), c.view(torch.uint8)) and torch.equal(exps[:, lo // 32:(hi + 31) // 32], e)
+        assert torch.equal(back[:, lo:hi], M.activation_unpack8(c, e, BF))
+
+
+# ---- missing parameters ------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("has_w,has_b", [(False, True), (True, False), (False, False)])
+@pytest.mark.parametrize("dtype,ptype", [(BF, BF), (HF, F32)])
+def test_layer_norm_gradients_with_a_missing_parameter(has_w, has_b, dtype, ptype):
+    """Each gradient that is there, and each of them alone."""
+    x, w, b, dy = ln_case(130, 300, dtype, ptype, 4)
+    w, b = w if has_w else None, b if has_b else None
+    y0, mean, rstd = FO.layer_norm(x, w, b, EPS)
+    t = ln_tolerances(x, w, b, dy, dtype, (mean, rstd))
+    want = dict(zip("xwb", zip(FO.layer_norm_backward(dy, x, w, mean, rstd), t[3:])))
+    there = ["x"] + ["w"] * has_w + ["b"] * has_b
+    for asked in [there] + [[n] for n in there]:
+        leaf = {n: None if v is None else v.cuda().requires_grad_(n in asked) for n, v in (("x", x), ("w", w), ("b", b))}
+        y = M.layer_norm(leaf["x"], leaf["w"], leaf["b"], EPS)
+        within(y, y0, t[0], "y")
+        for n, g in zip(asked, torch.autograd.grad(y, [leaf[n] for n in asked], dy.cuda())):
+            ref, tol = want[n]
+            assert g.dtype == leaf[n].dtype
+            within(g, ref, tol if n == "x" else tol + U[ptype] * ref.abs() + TINY[ptype], "d_" + n)
+
+
 # ---- forward-mode tangents ---------------------------------------------------------------------------------------------------
 
 def test_forward_mode_tangents_are_refused_not_lost():
