@@ -74,7 +74,8 @@ int hstu_hip_layer_norm_backward(const hstu_layer_norm_bwd_params* p, void* work
  *   code = float8_e4m3fn nearest to v * 2^-E (ties to even); NaN for NaN and infinities
  *   exponents[row, group] = E + 127
  * A code stands for code * 2^E, brought into the finite range of the type it is read in.  With power-of-two scales a value is
- * off by at most 2^-4 of itself or 2^-10 * 2^E, whichever is larger, and packing an unpacked tensor again changes nothing. */
+ * off by at most 2^-4 of itself or 2^-10 * 2^E, whichever is larger, and packing an unpacked tensor again changes no value.  (It may
+ * change the codes: a group whose largest value was rounded down to 224 * 2^E comes back with E - 1 and codes twice as large.) */
 #define HSTU_PACK8_GROUP 32
 #define HSTU_PACK8_MAX_COLS 65536
 typedef struct hstu_pack8_params {

@@ -6,6 +6,7 @@ import torch
 import torch.autograd.forward_ad as fwd_ad
 
 import recsdk_amd  # noqa: F401
+from oracle import ffn_oracle as FO
 from recsdk_amd import _capi
 from tests.ffn_cases import INSTANCES, described
 
@@ -60,3 +61,13 @@ def test_described_kernels():
     assert L.hstu_hip_gated_linear_backward_describe_kernel(None, buf, 8) == -1
     p.k = 0
     assert L.hstu_hip_gated_linear_describe_kernel(C.byref(p), buf, 8) == -1
+
+
+def test_packing_again_changes_no_value_but_may_change_the_codes():
+    """225 rounds down to 224 = 448 / 2, which the next exponent below holds."""
+    x = torch.tensor([[225.0, -13.0, 0.3, 2.0 ** -9, 100.0]])
+    vals, exps = FO.pack8(x)
+    back = FO.unpack8(vals, exps, torch.float32)
+    again, exps2 = FO.pack8(back)
+    assert float(vals[0, 0]) == 224.0 and int(exps[0, 0]) == 127 and float(again[0, 0]) == 448.0 and int(exps2[0, 0]) == 126
+    assert torch.equal(FO.unpack8(again, exps2, torch.float32), back) and torch.equal(again, 2 * vals)

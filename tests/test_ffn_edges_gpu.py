@@ -208,6 +208,21 @@ def test_pack8_of_the_widest_rows(cols):
         assert torch.equal(back[:, lo:hi], M.activation_unpack8(c, e, BF))
 
 
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+def test_packing_again_changes_no_value(dtype):
+    """Groups whose largest value is rounded down to half of the largest code come back with other codes for the same values."""
+    g = torch.Generator().manual_seed(8)
+    x = (torch.randn(60, 96, generator=g) * torch.exp(2 * torch.randn(60, 1, generator=g))).to(dtype)
+    x[::3, ::32] = (x.float()[::3].abs().amax(dim=1, keepdim=True) * 4).to(dtype)      # (the largest of each group)
+    x[:30:3, ::32] = 225.0
+    codes, exps = M.activation_pack8(x.cuda())
+    back = M.activation_unpack8(codes, exps, dtype)
+    codes2, exps2 = M.activation_pack8(back)
+    assert torch.equal(M.activation_unpack8(codes2, exps2, dtype), back)
+    moved = exps2 != exps
+    assert bool(moved[:30:3].all()) and torch.equal(exps2[moved], exps[moved] - 1)
+
+
 # ---- missing parameters ------------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("has_w,has_b", [(False, True), (True, False), (False, False)])
