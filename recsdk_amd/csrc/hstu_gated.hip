@@ -4,8 +4,11 @@
 //             activation and product happen on the accumulators
 //   backward  dz from d_out and the kept z (24 bits; one pass, also the column sums for d_bias), then d_x = dz W and d_weight = dz^T x,
 //             which read their operands as they lie in memory (transposing LDS reads; nothing is transposed in HBM)
-// dz is rounded to the I/O type between the two: the products run on the 16-bit matrix cores, and the rounding (2^-9 relative
-// per element, independent) averages out over sums of 2 f and of m terms.
+// dz is rounded to the I/O type between the two, as any training in that type rounds it: the products run on the 16-bit matrix cores.
+// A rounding is off by at most 2^-8 (bf16) or 2^-11 (fp16) of the element and independent of the others; over sums of 2 f and of m terms
+// it comes out in the norm as large as the rounding of d_x and d_weight themselves.  16384 x 1024 -> 4096 bf16: the gradients are off
+// by 0.00234 of their norm, 0.00166 with dz in fp32 (fp16: 0.000293 and 0.000207).  dz in two 16-bit parts would take both products
+// twice, 500 us more of 940.
 #include <cstdio>
 
 #include "hstu_ffn_common.h"
@@ -199,8 +202,10 @@ struct Plan { int tile, splits, tiles_n, tiles_m; int64_t c_split; double us; };
 // beyond one cost a second kernel that adds their fp32 sums.
 // Measured (bf16, a full chip): a piece of a 256 x 256 tile 1.7, of a 256 x 128 one 1.1, of a 128 x 128 one 0.6 alone on its CU with
 // four buffers, 0.65 with two and 1.15 with two workgroups on a CU, of a 64 x 128 one 0.42 and 0.8.  fp32 products are bound by
-// their matrix rate: 128 x 128 x 32 in 1.8, 64 x 128 x 32 in 0.95.  Over 129 products of random sizes the choice is 0.3 % (forward), 0.8 %
-// (d_x) and 1.7 % (d_weight) slower than the fastest in the mean, 16 % at worst; fp32 0, 3.5 and 1.2 %.
+// their matrix rate: 128 x 128 x 32 in 1.8, 64 x 128 x 32 in 0.95.  Over 129 products of random sizes, each timed in every tile,
+// the choice is 0.3 % (forward), 0.8 % (d_x) and 1.5 % (d_weight) slower than the fastest in the mean, 12 % at worst; fp32 0, 3.5 and
+// 1.2 %, 16 % at worst.  The times themselves are rough where a launch is short: the fp32 forward of
+// 1123 x 240 -> 960 is reckoned 17.4 us in two tiles alike and takes 22 (26 with z kept).
 // Each tile has the sizes where it is the fastest (forward, us: 256 x 256, 128 x 128, 256 x 128, 64 x 128):
 //   2789 x 1008 x 2736 fp16 37 44 40 55;  16384 x 512 x 2048 bf16 90 91 87 109;  8000 x 128 x 512 bf16 10.4 7.5 7.5 9.0;
 //   256 x 1024 x 4096 bf16 26 12.4 16 9.2;  100 x 2000 x 4000 fp32 473 134 245 74

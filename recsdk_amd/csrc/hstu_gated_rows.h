@@ -6,9 +6,10 @@
 // operand); loaded as fragments, 16 rows to 16 neighbouring lanes, a load brings 16 bytes a cycle into a CU for 64.  Rows of any
 // alignment are read in place; what the last piece of a row has of them is cut out of the row's last 16 bytes.  The waves' fp32 sums
 // meet in LDS and are added in order.
-// Bounded by reading W, for more rows by each workgroup's reading of all of x.  1024 -> 4096 bf16: one row 3.4 us (16.8 MB of W, part of
-// it out of the caches; 4.2 loaded as fragments), 48 rows 4.7 (7.0); 4096 -> 1024: one row 6.0 (10.3), 64 rows 11.5 (24).  32 columns a
-// workgroup are slower (6.2 for 4.3 at one row), and so is a second piece under way.
+// Bounded by reading W, for more rows by each workgroup's reading of all of x: at 48 rows of 1024 -> 4096 the 256 workgroups fetch 25 MB of
+// x from the L2s beside 16.8 MB of W.  1024 -> 4096 bf16: one row 3.4 us (part of W out of the caches; 4.2 loaded as fragments), 48 rows
+// 4.7 (7.0); 4096 -> 1024: one row 6.0 (10.3), 64 rows 11.5 (24).  32 columns a workgroup, half the readers of x, are slower at one row (6.2
+// for 4.3; more rows were not measured), and so is a second piece under way.
 #pragma once
 #include "hstu_gemm.h"
 

@@ -15,8 +15,9 @@
 //
 // Bounded by the matrix cores once a product fills the chip: [8192, 8192] outputs over c = 8192 reach 1340 TFLOP/s in bf16, and
 // one large library product 1351.  Below that it is the start and the end of a tile that cost, 5 to 7 us per round of tiles: the
-// gated forward at 8192 x 1024 -> 2 * 4096, whose contraction is 16 pieces and whose end computes the activation, takes 124 to 132 us
-// (1110 to 1040 TFLOP/s), and its counters show the matrix cores busy for 45 % of it; 16384 rows with kept z take 303 us.
+// gated forward at 8192 x 1024 -> 2 * 4096, whose contraction is 16 pieces and whose end computes the activation, takes 124 to 134 us
+// (1110 to 1025 TFLOP/s; with GELU, whose 16 library erfc a block have nothing beside them there, 150 to 156), and its counters show the
+// matrix cores busy for 45 % of it; 16384 rows with kept z take 303 us.
 // Tried at that size and slower: four waves of 128 x 128 (263 us against 140 at the time: no second wave covers the end of the
 // first), the next lines called into L2 early (143), accumulators that start at the bias (145), workgroups that go on to their
 // next tile and start its copies before their end (140, and registers spilled).

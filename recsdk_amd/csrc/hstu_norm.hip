@@ -1,13 +1,15 @@
 // LayerNorm over the last axis, forward and backward (mxrec::layer_norm), any width up to 16384.  HBM-bound row work: a row
 // is held in the registers of LPR neighbouring lanes (8 to 64 of a wave, or a workgroup of 256 to 1024), NP pieces of 8
 // consecutive columns each, so that it is read once and the variance is taken from the deviations.  Rows of any width and
-// alignment take the same path: a lane's 16-byte accesses may start anywhere, only a row's last piece goes by elements.
+// alignment take the same path: a lane's 16-byte accesses may start anywhere, a row's last piece goes by four, two and one elements.
 //   forward   mean = sum x / C, var = sum (x - mean)^2 / C, rstd = 1 / sqrt(var + eps), y = (x - mean) rstd w + b
 //   backward  a = dy w, dx = rstd (a - (sum a + x_hat sum a x_hat) / C), dw = sum_rows dy x_hat, db = sum_rows dy
 // The column sums stay in registers over the rows that a lane sees, meet in LDS, leave as one row of partial sums per
 // workgroup, and a second kernel adds those in a fixed order: no atomics, reproducible.
+// Every finite row is taken: the sum is formed in units of 2^14 (an FMA in place of an addition, the same bits), and a row whose
+// squared deviations leave fp32, one that hardly ever comes, takes its variance from deviations in units of 2^90.
 // [262144, 512] bf16: forward 101 us (5.3 TB/s; a large copy 4.9), backward 137 to 143 (5.6 to 5.9), column sums 4.8.
-// Widths off the 8-column grid pay for accesses that straddle lines: [262144, 257] 86 and 161 us, [262144, 256] 54 and 70.
+// Widths off the 8-column grid pay for accesses that straddle lines: [262144, 257] 88 and 166 us, [262144, 256] 54 and 70.
 #include "hstu_ffn_common.h"
 
 namespace hstu {
